@@ -438,6 +438,78 @@ int mb_ipc_free(void* ptr);
 int mb_count_columns_noalloc(const int32_t* words, int64_t rows, int64_t n, int64_t* counts64,
                              int32_t* counts32, void* stream);
 
+/*
+ * Attention with a decay for each head over time-major steps:
+ *
+ *   forward (reverse = 0):  S_t = g S_{t-1} + kv_scale k_t v_t^T
+ *                           o_t = out_scale q_t^T S_t
+ *   reverse (reverse = 1):  G_t = H_{t+1} + kv_scale k_t v_t^T,  H_t = g G_t
+ *                           o_t = out_scale q_t^T G_t
+ *
+ * for every batch row b and head h, g = decay[h] (fp32, >= 0), t over the row's
+ * first lengths[b] steps (all T without lengths; values are clamped to [0, T]).
+ * `first` (optional, zeros without it) is S_{-1}, or H past the last step;
+ * `last` (optional) receives the final S, or H_0. Outputs at steps past the
+ * row's length are zero, and what the inputs hold there is not used.
+ * q, k: [T, B, H, Dk], v, o: [T, B, H, Dv] of `dtype`, element strides per step,
+ * row and head, contiguous along the head; first, last: fp32 [B, H, Dk, Dv] with
+ * four element strides. Head sizes 1..256. The three gradients are calls of the
+ * same function: dq from (do, v, k) forward, dk from (v, do, q) and dv from
+ * (k, q, do) in reverse.
+ * Sums and memories are fp32. The result does not depend on other rows.
+ * Workspace: mb_decay_attention_workspace_bytes(args) bytes (0 when the time axis
+ * is not split); calls that may overlap need their own.
+ * No counterpart in the reference.
+ */
+typedef struct mb_steps {
+  void* data;
+  int64_t stride_t, stride_b, stride_h;
+} mb_steps;
+
+typedef struct mb_memory {
+  float* data;
+  int64_t stride_b, stride_h, stride_row, stride_col;
+} mb_memory;
+
+typedef struct mb_decay_attention_args {
+  int dtype;
+  int reverse;
+  int64_t T, B, H, Dk, Dv;
+  mb_steps q, k, v, o;
+  const float* decay;
+  const int32_t* lengths;
+  mb_memory first, last;
+  float out_scale, kv_scale;
+} mb_decay_attention_args;
+
+int64_t mb_decay_attention_workspace_bytes(const mb_decay_attention_args* args);
+int mb_decay_attention(const mb_decay_attention_args* args, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/*
+ * One step of the forward recurrence over a batch of memories:
+ *   memory_out = g memory_in + k v^T,  o = scale q^T memory_out
+ * q, k: [B, H, Dk], v: [B, H, Dv] with element strides per row and head; o:
+ * contiguous [B, H, Dv]; memory_in, memory_out: contiguous fp32 [B, H, Dk, Dv],
+ * the same buffer or disjoint ones. active (optional, one byte per batch row): a
+ * row whose byte is 0 keeps its memory and gets zero outputs.
+ * No counterpart in the reference.
+ */
+typedef struct mb_decay_attention_step_args {
+  int dtype;
+  int64_t B, H, Dk, Dv;
+  const void *q, *k, *v;
+  void* o;
+  int64_t q_stride_b, q_stride_h, k_stride_b, k_stride_h, v_stride_b, v_stride_h;
+  const float* decay;
+  const float* memory_in;
+  float* memory_out;
+  const uint8_t* active;
+  float scale;
+} mb_decay_attention_step_args;
+
+int mb_decay_attention_step(const mb_decay_attention_step_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,6 +5,11 @@ modules, bit-packed spikes and their collectives. All compute runs in the
 hand-written CUDA library ``libmyelin_b200.so`` (see ``include/myelin_b200.h``).
 """
 
+from myelin_b200.attention import (
+    DecayAttentionState,
+    decay_attention_forward,
+    decay_attention_step,
+)
 from myelin_b200.checkpointing import (
     CheckpointPolicy,
     CheckpointSize,

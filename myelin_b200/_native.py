@@ -100,6 +100,9 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mb_pack_count_scatter": (
         _int, [_int, _vp, _vp, _i64, _i64, _vp, _int, _vp, _vp, _vp, _i64, _vp]
     ),
+    "mb_decay_attention_workspace_bytes": (_i64, [_vp]),
+    "mb_decay_attention": (_int, [_vp, _vp, _i64, _vp]),
+    "mb_decay_attention_step": (_int, [_vp, _vp]),
     "mb_ipc_handle_bytes": (_int, []),
     "mb_ipc_alloc": (_int, [_i64, _vp, _vp]),
     "mb_ipc_open": (_int, [_vp, _vp]),
@@ -538,3 +541,84 @@ def ipc_close(address: int) -> None:
 
 def ipc_free(address: int) -> None:
     check(lib().mb_ipc_free(address), "mb_ipc_free")
+
+
+class StepsC(ctypes.Structure):
+    """``mb_steps``: a [T, B, H, D] tensor, contiguous along D."""
+
+    _fields_ = [("data", _vp), ("stride_t", _i64), ("stride_b", _i64), ("stride_h", _i64)]
+
+    @classmethod
+    def of(cls, t: torch.Tensor) -> "StepsC":
+        st, sb, sh, _ = t.stride()
+        return cls(t.data_ptr(), st, sb, sh)
+
+
+class MemoryC(ctypes.Structure):
+    """``mb_memory``: an fp32 [B, H, rows, cols] tensor of any strides."""
+
+    _fields_ = [("data", _vp), ("stride_b", _i64), ("stride_h", _i64), ("stride_row", _i64),
+                ("stride_col", _i64)]
+
+    @classmethod
+    def of(cls, t: torch.Tensor | None) -> "MemoryC":
+        return cls() if t is None else cls(t.data_ptr(), *t.stride())
+
+
+class DecayAttentionArgsC(ctypes.Structure):
+    """``mb_decay_attention_args`` (include/myelin_b200.h)."""
+
+    _fields_ = [("dtype", _int), ("reverse", _int), ("T", _i64), ("B", _i64), ("H", _i64),
+                ("Dk", _i64), ("Dv", _i64), ("q", StepsC), ("k", StepsC), ("v", StepsC),
+                ("o", StepsC), ("decay", _vp), ("lengths", _vp), ("first", MemoryC),
+                ("last", MemoryC), ("out_scale", _f), ("kv_scale", _f)]
+
+
+class DecayAttentionStepArgsC(ctypes.Structure):
+    """``mb_decay_attention_step_args`` (include/myelin_b200.h)."""
+
+    _fields_ = [("dtype", _int), ("B", _i64), ("H", _i64), ("Dk", _i64), ("Dv", _i64),
+                ("q", _vp), ("k", _vp), ("v", _vp), ("o", _vp), ("q_stride_b", _i64),
+                ("q_stride_h", _i64), ("k_stride_b", _i64), ("k_stride_h", _i64),
+                ("v_stride_b", _i64), ("v_stride_h", _i64), ("decay", _vp), ("memory_in", _vp),
+                ("memory_out", _vp), ("active", _vp), ("scale", _f)]
+
+
+def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
+                    decay: torch.Tensor, lengths: torch.Tensor | None,
+                    first: torch.Tensor | None, last: torch.Tensor | None, *, reverse: bool,
+                    out_scale: float, kv_scale: float) -> None:
+    """``mb_decay_attention`` on [T, B, H, D] tensors that are contiguous along D;
+    ``first`` and ``last`` may have any strides (a transposed view included)."""
+
+    T, B, H, Dk = q.shape
+    args = DecayAttentionArgsC(
+        dtype_code(q.dtype), int(reverse), T, B, H, Dk, v.shape[3], StepsC.of(q), StepsC.of(k),
+        StepsC.of(v), StepsC.of(o), ptr(decay), ptr(lengths), MemoryC.of(first),
+        MemoryC.of(last), out_scale, kv_scale,
+    )
+    at = ctypes.addressof(args)
+    with torch.cuda.device(q.device):
+        need = int(lib().mb_decay_attention_workspace_bytes(at))
+        if need < 0:
+            check(1, "mb_decay_attention")
+        ws = torch.empty(need // 4, dtype=torch.float32, device=q.device) if need > 0 else None
+        status = lib().mb_decay_attention(at, ptr(ws), need, stream_handle(q.device))
+    check(status, "mb_decay_attention")
+
+
+def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
+                         decay: torch.Tensor, memory_in: torch.Tensor, memory_out: torch.Tensor,
+                         active: torch.Tensor | None, scale: float) -> None:
+    """``mb_decay_attention_step`` on [B, H, D] tensors that are contiguous along D
+    and contiguous memories [B, H, Dk, Dv]."""
+
+    B, H, Dk = q.shape
+    args = DecayAttentionStepArgsC(
+        dtype_code(q.dtype), B, H, Dk, v.shape[2], ptr(q), ptr(k), ptr(v), ptr(o), q.stride(0),
+        q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), ptr(decay),
+        ptr(memory_in), ptr(memory_out), ptr(active), scale,
+    )
+    with torch.cuda.device(q.device):
+        status = lib().mb_decay_attention_step(ctypes.addressof(args), stream_handle(q.device))
+    check(status, "mb_decay_attention_step")

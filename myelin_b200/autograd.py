@@ -283,3 +283,32 @@ class TwoLayerPackedHiddenRateFunction(torch.autograd.Function):
             grad_w1, _ = _weight_bias_grads(x2, g1, w1, None, need_w1, False)
             grad_b1 = cops.bias_grad(outs1[3].view(B, H), b1) if sum1 else None
         return (grad_x, grad_w1, grad_b1, grad_w2, grad_b2, *tail)
+
+
+class DecayAttentionFunction(torch.autograd.Function):
+    """Attention with a decay for each head: (queries, keys, values, memory) ->
+    (outputs, final memory). Saves its inputs only; the backward runs the same
+    kernels on other operands and recomputes every score and memory
+    (``compile_ops.decay_attention_backward``).
+    """
+
+    @staticmethod
+    def forward(ctx: Any, q, k, v, decay, memory, lengths, scale: float):
+        out, last = cops.decay_attention(q, k, v, decay, memory, lengths, scale)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, v, decay, memory, lengths)
+        ctx.scale = scale
+        return out, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx: Any, g_out, g_last):
+        if g_out is None and g_last is None:
+            return (None,) * 7
+        q, k, v, decay, memory, lengths = ctx.saved_tensors
+        need_q, need_k, need_v, _, need_m = ctx.needs_input_grad[:5]
+        dq, dk, dv, dm = cops.decay_attention_backward(
+            q, k, v, decay, memory, lengths, g_out, g_last, ctx.scale, need_q=need_q,
+            need_k=need_k, need_v=need_v, need_first=need_m and memory is not None,
+        )
+        return dq, dk, dv, None, dm, None, None

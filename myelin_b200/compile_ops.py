@@ -488,6 +488,174 @@ def izhikevich_forward(x: torch.Tensor, v0: torch.Tensor, u0: torch.Tensor,
     return _izhikevich_impl(x, v0, u0, list(params))
 
 
+# ---------------------------------------------------------------------------
+# attention with a decay for each head
+# ---------------------------------------------------------------------------
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """The tensor itself when its last dimension is contiguous, else a copy."""
+
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _decay_attention_impl(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
+    first: torch.Tensor | None, lengths: torch.Tensor | None, scale: float,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    T, B, H, Dk = q.shape
+    Dv = v.shape[3]
+    out = torch.empty((T, B, H, Dv), dtype=q.dtype, device=q.device)
+    last = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device)
+    nat.decay_attention(_rows(q), _rows(k), _rows(v), out, decay, lengths, first, last,
+                        reverse=False, out_scale=scale, kv_scale=1.0)
+    return out, last
+
+
+decay_attention_op = torch.library.custom_op(f"{_NS}::decay_attention", _decay_attention_impl,
+                                             mutates_args=())
+
+
+@decay_attention_op.register_fake
+def _decay_attention_fake(q, k, v, decay, first, lengths, scale):
+    T, B, H, Dk = q.shape
+    Dv = v.shape[3]
+    return q.new_empty((T, B, H, Dv)), q.new_empty((B, H, Dk, Dv), dtype=torch.float32)
+
+
+def decay_attention(q, k, v, decay, first, lengths, scale):
+    """Chunked forward (``mb_decay_attention``): (outputs, final memory)."""
+
+    args = (q, k, v, decay, first, lengths, float(scale))
+    return decay_attention_op(*args) if _tracing() else _decay_attention_impl(*args)
+
+
+def _decay_attention_backward_eager(q, k, v, decay, first, lengths, grad_out, grad_last, scale,
+                                    need_q, need_k, need_v, need_first):
+    """Allocates only the requested gradients; the others are None. Each is the
+    operator itself on other operands: dq from (grad, v, k) forward, dk from
+    (v, grad, q) and dv from (k, q, grad) in reverse, whose final memory is the
+    initial memory's gradient."""
+
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    grad_out = (torch.zeros(v.shape, dtype=v.dtype, device=v.device) if grad_out is None
+                else _rows(grad_out))
+    dq = dk = dv = dfirst = None
+    if need_q:
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        nat.decay_attention(grad_out, v, k, dq, decay, lengths,
+                            None if first is None else first.transpose(-1, -2), None,
+                            reverse=False, out_scale=scale, kv_scale=1.0)
+    if need_k:
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        nat.decay_attention(v, grad_out, q, dk, decay, lengths,
+                            None if grad_last is None else grad_last.transpose(-1, -2), None,
+                            reverse=True, out_scale=1.0, kv_scale=scale)
+    if need_v or need_first:
+        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        if need_first:
+            T, B, H, Dk = q.shape
+            dfirst = torch.empty((B, H, Dk, v.shape[3]), dtype=torch.float32, device=q.device)
+        nat.decay_attention(k, q, grad_out, dv, decay, lengths, grad_last, dfirst, reverse=True,
+                            out_scale=1.0, kv_scale=scale)
+    return dq, dk, dv if need_v else None, dfirst
+
+
+def _decay_attention_backward_impl(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
+    first: torch.Tensor | None, lengths: torch.Tensor | None, grad_out: torch.Tensor | None,
+    grad_last: torch.Tensor | None, scale: float, need_q: bool, need_k: bool, need_v: bool,
+    need_first: bool,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    outs = _decay_attention_backward_eager(q, k, v, decay, first, lengths, grad_out, grad_last,
+                                           scale, need_q, need_k, need_v, need_first)
+    empty = (q.new_empty(0), q.new_empty(0), q.new_empty(0), q.new_empty(0, dtype=torch.float32))
+    return tuple(e if t is None else t for t, e in zip(outs, empty))  # type: ignore[return-value]
+
+
+decay_attention_backward_op = torch.library.custom_op(
+    f"{_NS}::decay_attention_backward", _decay_attention_backward_impl, mutates_args=())
+
+
+@decay_attention_backward_op.register_fake
+def _decay_attention_backward_fake(q, k, v, decay, first, lengths, grad_out, grad_last, scale,
+                                   need_q, need_k, need_v, need_first):
+    T, B, H, Dk = q.shape
+    return (q.new_empty(q.shape if need_q else (0,)), k.new_empty(k.shape if need_k else (0,)),
+            v.new_empty(v.shape if need_v else (0,)),
+            q.new_empty((B, H, Dk, v.shape[3]) if need_first else (0,), dtype=torch.float32))
+
+
+def decay_attention_backward(q, k, v, decay, first, lengths, grad_out, grad_last, scale, *,
+                             need_q=True, need_k=True, need_v=True, need_first=False):
+    """Gradients of ``decay_attention``: (dq, dk, dv, dfirst); those that were not
+    requested are None."""
+
+    args = (q, k, v, decay, first, lengths, grad_out, grad_last, float(scale), bool(need_q),
+            bool(need_k), bool(need_v), bool(need_first))
+    if _tracing():
+        return tuple(_none0(t) for t in decay_attention_backward_op(*args))
+    return _decay_attention_backward_eager(*args)
+
+
+def _decay_attention_step_impl(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
+    memory: torch.Tensor, active: torch.Tensor | None, scale: float,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    memory = memory.contiguous()
+    last = torch.empty_like(memory)
+    nat.decay_attention_step(_rows(q), _rows(k), _rows(v), out, decay, memory, last, active,
+                             scale)
+    return out, last
+
+
+decay_attention_step_op = torch.library.custom_op(
+    f"{_NS}::decay_attention_step", _decay_attention_step_impl, mutates_args=())
+
+
+@decay_attention_step_op.register_fake
+def _decay_attention_step_fake(q, k, v, decay, memory, active, scale):
+    return v.new_empty(v.shape), memory.new_empty(memory.shape)
+
+
+def decay_attention_step(q, k, v, decay, memory, active, scale):
+    """One step (``mb_decay_attention_step``): (outputs, new memory)."""
+
+    args = (q, k, v, decay, memory, active, float(scale))
+    return decay_attention_step_op(*args) if _tracing() else _decay_attention_step_impl(*args)
+
+
+def _decay_attention_step_inplace_impl(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
+    memory: torch.Tensor, active: torch.Tensor | None, scale: float,
+) -> torch.Tensor:
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    nat.decay_attention_step(_rows(q), _rows(k), _rows(v), out, decay, memory, memory, active,
+                             scale)
+    return out
+
+
+decay_attention_step_inplace_op = torch.library.custom_op(
+    f"{_NS}::decay_attention_step_", _decay_attention_step_inplace_impl, mutates_args=("memory",))
+
+
+@decay_attention_step_inplace_op.register_fake
+def _decay_attention_step_inplace_fake(q, k, v, decay, memory, active, scale):
+    return v.new_empty(v.shape)
+
+
+def decay_attention_step_(q, k, v, decay, memory, active, scale):
+    """One step with the memory updated in place: the outputs."""
+
+    args = (q, k, v, decay, memory, active, float(scale))
+    if _tracing():
+        return decay_attention_step_inplace_op(*args)
+    out = _decay_attention_step_inplace_impl(*args)
+    if not memory.is_inference():
+        torch.autograd.graph.increment_version(memory)  # as an in-place torch operation does
+    return out
+
+
 OPS = (scan_forward_op, scan_backward_op, gemm_tn_op, linear_project_op, linear_input_grad_op,
        linear_weight_grad_op, bias_grad_op, pack_op, unpack_op, count_rows_op, count_columns_op,
-       pack_count_op, izhikevich_op)
+       pack_count_op, izhikevich_op, decay_attention_op, decay_attention_backward_op,
+       decay_attention_step_op, decay_attention_step_inplace_op)
