@@ -510,6 +510,21 @@ typedef struct mb_decay_attention_step_args {
 
 int mb_decay_attention_step(const mb_decay_attention_step_args* args, void* stream);
 
+/*
+ * Dropout from a counter-based generator, the mask never stored:
+ *   y[e] = x[e] * 65536 / (65536 - threshold) if draw(e) >= threshold, else 0
+ * over `rows` rows of n contiguous elements of `dtype` (f32, bf16, f16) that
+ * share one mask (rows = 1: every element its own draw). draw(e), e the place in
+ * a row, is 16 bits of Philox 4x32-10 with key seed[0] and counter (e / 8,
+ * seed[1]): half e % 2 of word (e % 8) / 2. seed: two int64 in device memory,
+ * read when the kernel runs. threshold in [0, 65536]. y may be x. The gradient is
+ * the same call on the output's gradient.
+ * Replaces: nn.Dropout in RateReadoutClassifier (src/myelin/modules.py:848-903),
+ *   where a mask without storage, or one for all time steps, is wanted.
+ */
+int mb_dropout(int dtype, const void* x, void* y, int64_t rows, int64_t n, int threshold,
+               const int64_t* seed, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

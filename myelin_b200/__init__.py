@@ -25,6 +25,7 @@ from myelin_b200.distributed import (
     packed_spike_count_all_reduce,
     packed_spike_rate_all_reduce,
 )
+from myelin_b200.dropout import spike_dropout
 from myelin_b200.kernels import (
     Backend,
     alif_forward,
@@ -51,6 +52,7 @@ from myelin_b200.modules import (
     LinearSurrogateLIFRate,
     LinearSynapse,
     RateReadoutClassifier,
+    SpikeDropout,
     SurrogateALIFCell,
     SurrogateLIFCell,
     TimeUnroll,

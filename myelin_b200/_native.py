@@ -103,6 +103,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mb_decay_attention_workspace_bytes": (_i64, [_vp]),
     "mb_decay_attention": (_int, [_vp, _vp, _i64, _vp]),
     "mb_decay_attention_step": (_int, [_vp, _vp]),
+    "mb_dropout": (_int, [_int, _vp, _vp, _i64, _i64, _int, _vp, _vp]),
     "mb_ipc_handle_bytes": (_int, []),
     "mb_ipc_alloc": (_int, [_i64, _vp, _vp]),
     "mb_ipc_open": (_int, [_vp, _vp]),
@@ -622,3 +623,13 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
     with torch.cuda.device(q.device):
         status = lib().mb_decay_attention_step(ctypes.addressof(args), stream_handle(q.device))
     check(status, "mb_decay_attention_step")
+
+
+def dropout(x: torch.Tensor, y: torch.Tensor, rows: int, n: int, threshold: int,
+            seed: torch.Tensor) -> None:
+    """``mb_dropout`` over contiguous ``x[rows, n]``, one mask for all rows."""
+
+    with torch.cuda.device(x.device):
+        status = lib().mb_dropout(dtype_code(x.dtype), ptr(x), ptr(y), rows, n, threshold,
+                                  ptr(seed), stream_handle(x.device))
+    check(status, "mb_dropout")

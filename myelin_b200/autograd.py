@@ -312,3 +312,19 @@ class DecayAttentionFunction(torch.autograd.Function):
             need_k=need_k, need_v=need_v, need_first=need_m and memory is not None,
         )
         return dq, dk, dv, None, dm, None, None
+
+
+class DropoutFunction(torch.autograd.Function):
+    """Dropout that saves its seed, not its mask: the backward is the same
+    (linear) operator on the gradient, so it can be differentiated again."""
+
+    @staticmethod
+    def forward(ctx: Any, x, seed, threshold: int, time_shared: bool):
+        ctx.save_for_backward(seed)
+        ctx.cfg = (threshold, time_shared)
+        return cops.dropout(x, seed, threshold, time_shared)
+
+    @staticmethod
+    def backward(ctx: Any, g):
+        (seed,) = ctx.saved_tensors
+        return DropoutFunction.apply(g, seed, *ctx.cfg), None, None, None

@@ -655,7 +655,36 @@ def decay_attention_step_(q, k, v, decay, memory, active, scale):
     return out
 
 
+# ---------------------------------------------------------------------------
+# dropout
+# ---------------------------------------------------------------------------
+def _dropout_impl(x: torch.Tensor, seed: torch.Tensor, threshold: int,
+                  time_shared: bool) -> torch.Tensor:
+    x = x.contiguous()
+    y = torch.empty_like(x)
+    rows = x.shape[0] if time_shared else 1
+    if x.numel() > 0:
+        nat.dropout(x, y, rows, x.numel() // rows, threshold, seed)
+    return y
+
+
+dropout_op = torch.library.custom_op(f"{_NS}::dropout", _dropout_impl, mutates_args=())
+
+
+@dropout_op.register_fake
+def _dropout_fake(x, seed, threshold, time_shared):
+    return x.new_empty(x.shape)
+
+
+def dropout(x: torch.Tensor, seed: torch.Tensor, threshold: int,
+            time_shared: bool) -> torch.Tensor:
+    """Dropout with the mask of (seed, offset) = ``seed`` (``mb_dropout``)."""
+
+    args = (x, seed, int(threshold), bool(time_shared))
+    return dropout_op(*args) if _tracing() else _dropout_impl(*args)
+
+
 OPS = (scan_forward_op, scan_backward_op, gemm_tn_op, linear_project_op, linear_input_grad_op,
        linear_weight_grad_op, bias_grad_op, pack_op, unpack_op, count_rows_op, count_columns_op,
        pack_count_op, izhikevich_op, decay_attention_op, decay_attention_backward_op,
-       decay_attention_step_op, decay_attention_step_inplace_op)
+       decay_attention_step_op, decay_attention_step_inplace_op, dropout_op)

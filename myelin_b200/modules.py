@@ -16,6 +16,7 @@ import torch
 from torch import nn
 
 from myelin_b200.checkpointing import CheckpointSize
+from myelin_b200.dropout import spike_dropout
 from myelin_b200.kernels import (
     izhikevich_step,
     Backend,
@@ -324,8 +325,43 @@ class LinearSurrogateLIFRate(nn.Module):
         return rates
 
 
+class SpikeDropout(nn.Module):
+    """``spike_dropout`` with its own seed and a count of its calls.
+
+    ``rng`` (int64 buffer: seed, calls so far) moves and is saved with the
+    module; each call in training mode takes the next offset on the device, so a
+    captured graph draws a new mask at every replay. With ``time_shared`` (the
+    default) all steps of a ``[T, ...]`` input use one mask.
+    """
+
+    def __init__(self, p: float = 0.5, *, time_shared: bool = True,
+                 seed: int | None = None) -> None:
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"dropout probability must be in [0, 1]; got {p}")
+        self.p = p
+        self.time_shared = time_shared
+        first = int(torch.randint(2**62, ())) if seed is None else seed
+        self.register_buffer("rng", torch.tensor([first, 0], dtype=torch.int64))
+        self.register_buffer("_next", torch.tensor([0, 1], dtype=torch.int64), persistent=False)
+
+    def forward(self, inputs: torch.Tensor) -> torch.Tensor:
+        if not self.training or self.p == 0.0:
+            return inputs
+        seed = self.rng.clone()  # this call's own: its backward draws from it again
+        self.rng.add_(self._next)
+        return spike_dropout(inputs, self.p, seed, time_shared=self.time_shared)
+
+    def extra_repr(self) -> str:
+        return f"p={self.p}, time_shared={self.time_shared}"
+
+
 class RateReadoutClassifier(nn.Module):
-    """Hidden streamed LIF layer plus a rate readout (src/myelin/modules.py:848-903)."""
+    """Hidden streamed LIF layer plus a rate readout (src/myelin/modules.py:848-903).
+
+    ``time_shared_dropout`` drops hidden neurons for the whole window
+    (``SpikeDropout``) instead of per step (``nn.Dropout``).
+    """
 
     def __init__(
         self,
@@ -341,6 +377,7 @@ class RateReadoutClassifier(nn.Module):
         backend: Backend = "torch",
         checkpoint_size: CheckpointSize = 25,
         dropout: float = 0.0,
+        time_shared_dropout: bool = False,
     ) -> None:
         super().__init__()
         self.hidden = LinearSurrogateLIF(
@@ -355,7 +392,7 @@ class RateReadoutClassifier(nn.Module):
             stream_synapse=True,
             checkpoint_size=checkpoint_size,
         )
-        self.dropout = nn.Dropout(dropout)
+        self.dropout = SpikeDropout(dropout) if time_shared_dropout else nn.Dropout(dropout)
         self.output = LinearSurrogateLIFRate(
             hidden_features,
             out_features,
