@@ -92,7 +92,7 @@ const char* mb_version(void);
 int mb_device_status(int clear);
 
 /* Code units whose status words mb_device_status combines. */
-enum mb_unit { MB_UNIT_SCAN = 0, MB_UNIT_SCAN_FAST = 1, MB_UNIT_GEMM = 2 };
+enum mb_unit { MB_UNIT_SCAN = 0, MB_UNIT_SCAN_FAST = 1, MB_UNIT_GEMM = 2, MB_UNIT_GEMM_I8 = 3 };
 
 /* Diagnostic: launch one tiny kernel in `unit` whose single bounded wait
  * (budget `polls`, 1..65536) is on a barrier nothing arrives at, so it runs
@@ -524,6 +524,42 @@ int mb_decay_attention_step(const mb_decay_attention_step_args* args, void* stre
  */
 int mb_dropout(int dtype, const void* x, void* y, int64_t rows, int64_t n, int threshold,
                const int64_t* seed, void* stream);
+
+/*
+ * Rows quantised to signed 8-bit integers (symmetric, -127..127):
+ *   scale[r] = max|x[r, :]| / 127,  q = round(x * (127 / max|x[r, :]|)), ties to even
+ * x: `rows` rows of `cols` elements of `dtype` (f32, bf16, f16), ldx elements
+ * apart; q: ldq bytes apart; scale: fp32. A row whose largest magnitude is below
+ * 1e-30 gives zeros with scale 0; a row that holds an infinity or NaN gives zeros
+ * with scale NaN, so that everything computed from it is NaN.
+ * No counterpart in the reference.
+ */
+int mb_quantize_rows(int dtype, const void* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* q,
+                     int64_t ldq, float* scale, void* stream);
+
+/*
+ * C[m, n] = a_scale[m] b_scale[n] sum_k A[m, k] B[n, k] (+ bias[n])
+ * A [M, K], B [N, K] signed 8-bit rows lda, ldb bytes apart (multiples of 16, bases
+ * on 16 bytes; bytes between K and the pitch are not used), K < 2^17 so that every
+ * sum is exact in int32; a_scale fp32 [M] or NULL (1: integers, 0/1 spikes), b_scale
+ * fp32 [N], bias [N] of `bias_dtype` or NULL; C of `out_dtype` (f32, bf16, f16), rows
+ * ldc elements apart. One fp32 scaling, one rounding. tcgen05.mma kind::i8.
+ * Replaces: LinearSynapse's projection (src/myelin/modules.py:112-133) for inference.
+ */
+int mb_gemm_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* b, int64_t ldb,
+               const float* b_scale, const void* bias, int bias_dtype, int out_dtype, void* c,
+               int64_t ldc, int64_t M, int64_t N, int64_t K, void* stream);
+
+/*
+ * The same product for a few rows (mb_linear_i8_rows_supported(M, K)), whose rows
+ * are quantised inside the kernel as mb_quantize_rows does: x of `dtype` f32, bf16
+ * or f16; or MB_U8: signed 8-bit integers with x_scale fp32 [M] or NULL (1).
+ */
+int mb_linear_i8_rows_supported(int64_t M, int64_t K);
+int mb_linear_i8_rows(int dtype, const void* x, int64_t ldx, const float* x_scale, const int8_t* w,
+                      int64_t ldw, const float* w_scale, const void* bias, int bias_dtype,
+                      int out_dtype, void* c, int64_t ldc, int64_t M, int64_t N, int64_t K,
+                      void* stream);
 
 #ifdef __cplusplus
 }

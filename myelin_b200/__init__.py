@@ -51,11 +51,13 @@ from myelin_b200.modules import (
     LinearSurrogateLIFPacked,
     LinearSurrogateLIFRate,
     LinearSynapse,
+    QuantizedLinearSynapse,
     RateReadoutClassifier,
     SpikeDropout,
     SurrogateALIFCell,
     SurrogateLIFCell,
     TimeUnroll,
+    quantize_synapses,
 )
 from myelin_b200.neurons import (
     ALIFParams,
@@ -79,6 +81,13 @@ from myelin_b200.packing import (
     packed_spike_rate,
     spike_compression_ratio,
     unpack_spikes,
+)
+from myelin_b200.quantized import (
+    QuantizedRows,
+    QuantizedWeight,
+    quantize_rows,
+    quantize_weight,
+    quantized_linear,
 )
 from myelin_b200.surrogates import (
     SURROGATE_NAMES,

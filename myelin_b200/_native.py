@@ -104,6 +104,15 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mb_decay_attention": (_int, [_vp, _vp, _i64, _vp]),
     "mb_decay_attention_step": (_int, [_vp, _vp]),
     "mb_dropout": (_int, [_int, _vp, _vp, _i64, _i64, _int, _vp, _vp]),
+    "mb_quantize_rows": (_int, [_int, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "mb_gemm_i8": (
+        _int, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _int, _int, _vp, _i64, _i64, _i64, _i64, _vp]
+    ),
+    "mb_linear_i8_rows_supported": (_int, [_i64, _i64]),
+    "mb_linear_i8_rows": (
+        _int, [_int, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _int, _int, _vp, _i64, _i64, _i64, _i64,
+               _vp]
+    ),
     "mb_ipc_handle_bytes": (_int, []),
     "mb_ipc_alloc": (_int, [_i64, _vp, _vp]),
     "mb_ipc_open": (_int, [_vp, _vp]),
@@ -177,7 +186,7 @@ def device_status(clear: bool = True) -> int:
 
 
 # enum mb_unit: the code units whose status words mb_device_status combines
-MB_UNIT_SCAN, MB_UNIT_SCAN_FAST, MB_UNIT_GEMM = 0, 1, 2
+MB_UNIT_SCAN, MB_UNIT_SCAN_FAST, MB_UNIT_GEMM, MB_UNIT_GEMM_I8 = 0, 1, 2, 3
 
 
 def debug_wait_timeout(unit: int, polls: int = 256, device: torch.device | None = None) -> None:
@@ -633,3 +642,48 @@ def dropout(x: torch.Tensor, y: torch.Tensor, rows: int, n: int, threshold: int,
         status = lib().mb_dropout(dtype_code(x.dtype), ptr(x), ptr(y), rows, n, threshold,
                                   ptr(seed), stream_handle(x.device))
     check(status, "mb_dropout")
+
+
+def quantize_rows(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
+    """``mb_quantize_rows``: int8 ``q[M, K]`` and fp32 ``scale[M]`` of ``x[M, K]``
+    (rows contiguous along K, any pitch)."""
+
+    with torch.cuda.device(x.device):
+        status = lib().mb_quantize_rows(dtype_code(x.dtype), ptr(x), x.shape[0], x.shape[1],
+                                        x.stride(0), ptr(q), q.stride(0), ptr(scale),
+                                        stream_handle(x.device))
+    check(status, "mb_quantize_rows")
+
+
+def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor | None, b: torch.Tensor,
+            b_scale: torch.Tensor, bias: torch.Tensor | None, out: torch.Tensor) -> None:
+    """``mb_gemm_i8``: int8 ``a[M, K]``, ``b[N, K]`` with 16-byte row pitches."""
+
+    M, K = a.shape
+    N = b.shape[0]
+    with torch.cuda.device(a.device):
+        status = lib().mb_gemm_i8(
+            ptr(a), a.stride(0), ptr(a_scale), ptr(b), b.stride(0), ptr(b_scale), ptr(bias),
+            dtype_code(bias.dtype) if bias is not None else 0, dtype_code(out.dtype), ptr(out),
+            out.stride(0), M, N, K, stream_handle(a.device),
+        )
+    check(status, "mb_gemm_i8")
+
+
+# mb_linear_i8_rows: rows and staged bytes it takes (mb_linear_i8_rows_supported)
+I8_ROWS, I8_ROWS_BYTES = 4, 32 * 1024
+
+
+def linear_i8_rows(x: torch.Tensor, x_scale: torch.Tensor | None, w: torch.Tensor,
+                   w_scale: torch.Tensor, bias: torch.Tensor | None, out: torch.Tensor) -> None:
+    """``mb_linear_i8_rows``: a few rows ``x[M, K]`` (float, or int8 / bool) by int8 ``w[N, K]``."""
+
+    M, K = x.shape
+    with torch.cuda.device(x.device):
+        status = lib().mb_linear_i8_rows(
+            dtype_code(x.dtype), ptr(x), x.stride(0), ptr(x_scale), ptr(w), w.stride(0),
+            ptr(w_scale), ptr(bias), dtype_code(bias.dtype) if bias is not None else 0,
+            dtype_code(out.dtype), ptr(out), out.stride(0), M, w.shape[0], K,
+            stream_handle(x.device),
+        )
+    check(status, "mb_linear_i8_rows")

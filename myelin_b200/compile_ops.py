@@ -684,7 +684,94 @@ def dropout(x: torch.Tensor, seed: torch.Tensor, threshold: int,
     return dropout_op(*args) if _tracing() else _dropout_impl(*args)
 
 
+# ---------------------------------------------------------------------------
+# projection in 8-bit integers
+# ---------------------------------------------------------------------------
+def _pitched(rows: int, cols: int, device: torch.device) -> torch.Tensor:
+    """int8 [rows, cols] whose rows start on 16-byte boundaries."""
+
+    return torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :cols]
+
+
+def _quantize_rows_eager(x2: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    x2 = _rows(x2)
+    q = _pitched(*x2.shape, x2.device)
+    scale = torch.empty((x2.shape[0],), dtype=torch.float32, device=x2.device)
+    nat.quantize_rows(x2, q, scale)
+    return q, scale
+
+
+def _quantize_rows_impl(x2: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    q, scale = _quantize_rows_eager(x2)
+    return q.contiguous(), scale
+
+
+quantize_rows_op = torch.library.custom_op(f"{_NS}::quantize_rows", _quantize_rows_impl,
+                                           mutates_args=())
+
+
+@quantize_rows_op.register_fake
+def _quantize_rows_fake(x2):
+    return (x2.new_empty(x2.shape, dtype=torch.int8),
+            x2.new_empty((x2.shape[0],), dtype=torch.float32))
+
+
+def quantize_rows(x2: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """int8 values and fp32 scale of each row of ``x2[M, K]`` (``mb_quantize_rows``)."""
+
+    return quantize_rows_op(x2) if _tracing() else _quantize_rows_eager(x2)
+
+
+def _i8_operand(t: torch.Tensor) -> torch.Tensor:
+    """An int8 matrix whose rows the tensor-map copies can read: itself, or a copy."""
+
+    if t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1] \
+            and t.data_ptr() % 16 == 0:
+        return t
+    return _pitched(*t.shape, t.device).copy_(t)
+
+
+def _quantized_project_impl(x2: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.Tensor,
+                            weight_scale: torch.Tensor, bias: torch.Tensor | None,
+                            out_dtype: torch.dtype) -> torch.Tensor:
+    M, K = x2.shape
+    N = weight.shape[0]
+    out = torch.empty((M, N), dtype=out_dtype, device=x2.device)
+    if M == 0 or N == 0:
+        return out
+    if x2.dtype == torch.bool:
+        x2 = x2.view(torch.int8)
+    weight = _i8_operand(weight)
+    if M <= nat.I8_ROWS and M * ((K + 15) // 16 * 16) <= nat.I8_ROWS_BYTES:
+        nat.linear_i8_rows(_rows(x2), x_scale, weight, weight_scale, bias, out)
+        return out
+    if x2.dtype.is_floating_point:
+        x2, x_scale = _quantize_rows_eager(x2)
+    nat.gemm_i8(_i8_operand(x2), x_scale, weight, weight_scale, bias, out)
+    return out
+
+
+quantized_project_op = torch.library.custom_op(f"{_NS}::quantized_project",
+                                               _quantized_project_impl, mutates_args=())
+
+
+@quantized_project_op.register_fake
+def _quantized_project_fake(x2, x_scale, weight, weight_scale, bias, out_dtype):
+    return x2.new_empty((x2.shape[0], weight.shape[0]), dtype=out_dtype)
+
+
+def quantized_project(x2: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.Tensor,
+                      weight_scale: torch.Tensor, bias: torch.Tensor | None,
+                      out_dtype: torch.dtype) -> torch.Tensor:
+    """``x2[M, K]`` (float: quantised by rows; int8 / bool: as it is, times
+    ``x_scale``) by int8 ``weight[N, K]`` (``mb_gemm_i8``, ``mb_linear_i8_rows``)."""
+
+    args = (x2, x_scale, weight, weight_scale, bias, out_dtype)
+    return quantized_project_op(*args) if _tracing() else _quantized_project_impl(*args)
+
+
 OPS = (scan_forward_op, scan_backward_op, gemm_tn_op, linear_project_op, linear_input_grad_op,
        linear_weight_grad_op, bias_grad_op, pack_op, unpack_op, count_rows_op, count_columns_op,
        pack_count_op, izhikevich_op, decay_attention_op, decay_attention_backward_op,
-       decay_attention_step_op, decay_attention_step_inplace_op, dropout_op)
+       decay_attention_step_op, decay_attention_step_inplace_op, dropout_op, quantize_rows_op,
+       quantized_project_op)

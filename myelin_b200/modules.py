@@ -37,6 +37,7 @@ from myelin_b200.neurons import (
     LIFState,
 )
 from myelin_b200.packing import PackedSpikes
+from myelin_b200.quantized import QuantizedWeight, quantize_weight, quantized_linear
 from myelin_b200.surrogates import (
     SurrogateFn,
     atan_surrogate,
@@ -71,6 +72,39 @@ class LinearSynapse(nn.Module):
         if self.bias is not None:
             output = output + self.bias
         return output
+
+
+class QuantizedLinearSynapse(nn.Module):
+    """A ``LinearSynapse`` for inference in 8-bit integers (``quantized_linear``).
+
+    Holds the weight as int8 with one scale per output neuron; float inputs are
+    quantised by rows on the way in, bool and int8 spikes are taken as they are.
+    Spikes given as bool come out in the bias's dtype (float32 without a bias).
+    """
+
+    def __init__(self, weight: QuantizedWeight, bias: torch.Tensor | None = None) -> None:
+        super().__init__()
+        self.register_buffer("data", weight.data)
+        self.register_buffer("scale", weight.scale)
+        self.register_buffer("bias", None if bias is None else bias.detach().clone())
+
+    @classmethod
+    def from_synapse(cls, synapse: LinearSynapse) -> "QuantizedLinearSynapse":
+        return cls(quantize_weight(synapse.weight.detach()), synapse.bias)
+
+    def _apply(self, fn, recurse=True):
+        # a change of dtype is for the bias; the scales stay fp32
+        scale = self.scale
+        super()._apply(fn, recurse)
+        self.scale = scale.to(self.scale.device)
+        return self
+
+    def forward(self, inputs: torch.Tensor) -> torch.Tensor:
+        weight = QuantizedWeight(self.data, self.scale)
+        out_dtype = None
+        if not inputs.dtype.is_floating_point and self.bias is not None:
+            out_dtype = self.bias.dtype
+        return quantized_linear(inputs, weight, self.bias, out_dtype=out_dtype)
 
 
 class LIFCell(nn.Module):
@@ -269,7 +303,7 @@ class LinearSurrogateLIF(nn.Module):
 
     def forward(self, inputs: torch.Tensor) -> torch.Tensor:
         cell = self.unroll.cell
-        if self.stream_synapse:
+        if self.stream_synapse and isinstance(self.synapse, LinearSynapse):
             _state, spikes = linear_surrogate_lif_forward(
                 inputs,
                 self.synapse.weight,
@@ -445,3 +479,15 @@ class LinearSurrogateLIFPacked(nn.Module):
             checkpoint_size=self.checkpoint_size,
         )
         return packed
+
+
+def quantize_synapses(module: nn.Module) -> nn.Module:
+    """Replace the synapses of every ``LinearLIF`` and ``LinearSurrogateLIF`` in
+    ``module`` (itself included) by 8-bit ones, in place, for inference; returns
+    ``module``. Rate readouts and packed layers keep theirs: their projection is
+    part of a fused function that takes float weights."""
+
+    for m in module.modules():
+        if isinstance(m, LinearLIF | LinearSurrogateLIF) and isinstance(m.synapse, LinearSynapse):
+            m.synapse = QuantizedLinearSynapse.from_synapse(m.synapse)
+    return module
