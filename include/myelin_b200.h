@@ -92,7 +92,13 @@ const char* mb_version(void);
 int mb_device_status(int clear);
 
 /* Code units whose status words mb_device_status combines. */
-enum mb_unit { MB_UNIT_SCAN = 0, MB_UNIT_SCAN_FAST = 1, MB_UNIT_GEMM = 2, MB_UNIT_GEMM_I8 = 3 };
+enum mb_unit {
+  MB_UNIT_SCAN = 0,
+  MB_UNIT_SCAN_FAST = 1,
+  MB_UNIT_GEMM = 2,
+  MB_UNIT_GEMM_I8 = 3,
+  MB_UNIT_ATTENTION = 4
+};
 
 /* Diagnostic: launch one tiny kernel in `unit` whose single bounded wait
  * (budget `polls`, 1..65536) is on a barrier nothing arrives at, so it runs

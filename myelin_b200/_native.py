@@ -186,7 +186,7 @@ def device_status(clear: bool = True) -> int:
 
 
 # enum mb_unit: the code units whose status words mb_device_status combines
-MB_UNIT_SCAN, MB_UNIT_SCAN_FAST, MB_UNIT_GEMM, MB_UNIT_GEMM_I8 = 0, 1, 2, 3
+MB_UNIT_SCAN, MB_UNIT_SCAN_FAST, MB_UNIT_GEMM, MB_UNIT_GEMM_I8, MB_UNIT_ATTENTION = range(5)
 
 
 def debug_wait_timeout(unit: int, polls: int = 256, device: torch.device | None = None) -> None:

@@ -21,12 +21,14 @@ int scan_unit_status(bool clear);       // scan.cu
 int scan_fast_unit_status(bool clear);  // scan_fast.cu
 int gemm_unit_status(bool clear);       // gemm_tcgen05.cu
 int gemm_i8_unit_status(bool clear);    // gemm_i8.cu
+int attention_unit_status(bool clear);  // decay_attention_tc.cu
 
 // Launchers of each unit's wait-timeout probe (wait_timeout_probe_kernel).
 cudaError_t scan_unit_wait_probe(uint32_t polls, cudaStream_t stream);
 cudaError_t scan_fast_unit_wait_probe(uint32_t polls, cudaStream_t stream);
 cudaError_t gemm_unit_wait_probe(uint32_t polls, cudaStream_t stream);
 cudaError_t gemm_i8_unit_wait_probe(uint32_t polls, cudaStream_t stream);
+cudaError_t attention_unit_wait_probe(uint32_t polls, cudaStream_t stream);
 
 enum DeviceStatus : int {
   kStatusOk = 0,

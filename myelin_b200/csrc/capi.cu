@@ -30,17 +30,20 @@ int scan_unit_status(bool clear);
 int scan_fast_unit_status(bool clear);
 int gemm_unit_status(bool clear);
 int gemm_i8_unit_status(bool clear);
+int attention_unit_status(bool clear);
 cudaError_t scan_unit_wait_probe(uint32_t polls, cudaStream_t stream);
 cudaError_t scan_fast_unit_wait_probe(uint32_t polls, cudaStream_t stream);
 cudaError_t gemm_unit_wait_probe(uint32_t polls, cudaStream_t stream);
 cudaError_t gemm_i8_unit_wait_probe(uint32_t polls, cudaStream_t stream);
+cudaError_t attention_unit_wait_probe(uint32_t polls, cudaStream_t stream);
 }  // namespace mb
 
 // Every unit's word is read (and cleared when asked), so one call reports and
 // resets all of them; the first non-zero code in unit order is returned.
 extern "C" int mb_device_status(int clear) {
   int (*units[])(bool) = {mb::scan_unit_status, mb::scan_fast_unit_status,
-                          mb::gemm_unit_status, mb::gemm_i8_unit_status};
+                          mb::gemm_unit_status, mb::gemm_i8_unit_status,
+                          mb::attention_unit_status};
   int result = 0;
   bool failed = false;
   for (auto unit : units) {
@@ -64,6 +67,9 @@ extern "C" int mb_debug_wait_timeout(int unit, int polls, void* stream) {
     case MB_UNIT_GEMM: err = mb::gemm_unit_wait_probe(static_cast<uint32_t>(polls), s); break;
     case MB_UNIT_GEMM_I8:
       err = mb::gemm_i8_unit_wait_probe(static_cast<uint32_t>(polls), s);
+      break;
+    case MB_UNIT_ATTENTION:
+      err = mb::attention_unit_wait_probe(static_cast<uint32_t>(polls), s);
       break;
     default: mb::set_error("mb_debug_wait_timeout: unknown unit %d", unit); return 1;
   }

@@ -351,6 +351,17 @@ int launch_recurrent(const mb_decay_attention_args& a, const AttnSplit& split, b
   }
 }
 
+// The tensor-core kernel where its rules allow it, else the recurrent one.
+AttnSplit choose_split(const mb_decay_attention_args& a, bool tc) {
+  return tc ? attn_tc_split(a) : recurrent_split(a);
+}
+
+int launch_pass(const mb_decay_attention_args& a, const AttnSplit& split, bool tc,
+                bool states_only, cudaStream_t stream) {
+  return tc ? attn_tc_launch(a, split, states_only, stream)
+            : launch_recurrent(a, split, states_only, stream);
+}
+
 int64_t split_bytes(const mb_decay_attention_args& a, const AttnSplit& split) {
   return split.segments > 1 ? split.segments * a.B * a.H * a.Dk * a.Dv * int64_t(sizeof(float))
                             : 0;
@@ -386,7 +397,7 @@ extern "C" int64_t mb_decay_attention_workspace_bytes(const mb_decay_attention_a
   using namespace mb;
   if (check_args(args, "mb_decay_attention_workspace_bytes") != 0) return -1;
   if (args->B == 0 || args->H == 0) return 0;
-  return split_bytes(*args, recurrent_split(*args));
+  return split_bytes(*args, choose_split(*args, attn_tc_supported(*args)));
 }
 
 extern "C" int mb_decay_attention(const mb_decay_attention_args* args, void* workspace,
@@ -401,7 +412,8 @@ extern "C" int mb_decay_attention(const mb_decay_attention_args* args, void* wor
                             a.o.data != nullptr),
                "mb_decay_attention: q, k, v and o must not be null");
   if (a.T == 0 && a.last.data == nullptr) return 0;
-  AttnSplit split = recurrent_split(a);
+  const bool tc = attn_tc_supported(a);
+  AttnSplit split = choose_split(a, tc);
   const int64_t need = split_bytes(a, split);
   MB_CHECK_ARG(need <= workspace_bytes && (need == 0 || workspace != nullptr),
                "mb_decay_attention: workspace of %lld bytes, %lld needed",
@@ -409,14 +421,14 @@ extern "C" int mb_decay_attention(const mb_decay_attention_args* args, void* wor
   split.states = static_cast<float*>(workspace);
   cudaStream_t s = as_stream(stream);
   if (split.segments > 1) {
-    if (const int rc = launch_recurrent(a, split, true, s)) return rc;
+    if (const int rc = launch_pass(a, split, tc, true, s)) return rc;
     const int64_t total = a.B * a.H * a.Dk * a.Dv;
     const int64_t blocks = ceil_div(total, 256);
     MB_CHECK_ARG(blocks <= 0x7fffffff, "mb_decay_attention: too many memory elements");
     attn_segment_scan_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(a, split);
     MB_CHECK_LAUNCH("mb_decay_attention (segment scan)");
   }
-  return launch_recurrent(a, split, false, s);
+  return launch_pass(a, split, tc, false, s);
 }
 
 extern "C" int mb_decay_attention_step(const mb_decay_attention_step_args* args, void* stream) {

@@ -20,6 +20,7 @@ import pytest
 import torch
 
 import myelin_b200 as mb
+from myelin_b200 import _native as nat
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -420,3 +421,10 @@ def test_inference_mode_and_versions():
     mb.decay_attention_step(q, q, q, _decay(H), mb.DecayAttentionState(m), inplace=True)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_wait_timeout_is_reported():
+    nat.device_status()
+    nat.debug_wait_timeout(nat.MB_UNIT_ATTENTION)
+    torch.cuda.synchronize()
+    assert nat.device_status() == 1 and nat.device_status() == 0
