@@ -357,9 +357,9 @@ AttnSplit choose_split(const mb_decay_attention_args& a, bool tc) {
 }
 
 int launch_pass(const mb_decay_attention_args& a, const AttnSplit& split, bool tc,
-                bool states_only, cudaStream_t stream) {
-  return tc ? attn_tc_launch(a, split, states_only, stream)
-            : launch_recurrent(a, split, states_only, stream);
+                bool states, cudaStream_t stream) {
+  return tc ? attn_tc_launch(a, split, states, stream)
+            : launch_recurrent(a, split, states, stream);
 }
 
 int64_t split_bytes(const mb_decay_attention_args& a, const AttnSplit& split) {
@@ -420,8 +420,13 @@ extern "C" int mb_decay_attention(const mb_decay_attention_args* args, void* wor
                static_cast<long long>(workspace_bytes), static_cast<long long>(need));
   split.states = static_cast<float*>(workspace);
   cudaStream_t s = as_stream(stream);
-  if (split.segments > 1) {
+  // the tensor-core kernel for outputs keeps no exact memory: the final one comes
+  // from the states kernel, which also starts a split time axis
+  const bool states = split.segments > 1 || (tc && a.last.data != nullptr);
+  if (states) {
     if (const int rc = launch_pass(a, split, tc, true, s)) return rc;
+  }
+  if (split.segments > 1) {
     const int64_t total = a.B * a.H * a.Dk * a.Dv;
     const int64_t blocks = ceil_div(total, 256);
     MB_CHECK_ARG(blocks <= 0x7fffffff, "mb_decay_attention: too many memory elements");

@@ -45,10 +45,11 @@ __device__ __forceinline__ float decay_pow(float log2g, int64_t n) {
   return n == 0 ? 1.0f : exp2f(static_cast<float>(n) * log2g);
 }
 
-// Whether the tensor-core kernel takes these arguments, and its launches.
+// Whether the tensor-core kernels take these arguments, and their launches: `states`
+// (memories only; with one segment from `first` to `last`) or the outputs.
 bool attn_tc_supported(const mb_decay_attention_args& a);
 AttnSplit attn_tc_split(const mb_decay_attention_args& a);
-int attn_tc_launch(const mb_decay_attention_args& a, const AttnSplit& split, bool states_only,
+int attn_tc_launch(const mb_decay_attention_args& a, const AttnSplit& split, bool states,
                    cudaStream_t stream);
 
 }  // namespace mb

@@ -1,25 +1,30 @@
 // Attention with a decay for each head in chunks of 128 steps on the tensor
-// cores (formulas: decay_attention.cuh). One CTA walks the chunks of one
-// (batch row, head, segment); with S the carry, per chunk
+// cores (formulas: decay_attention.cuh). Two kernels, both one persistent CTA per
+// SM that walks whole (segment, batch row, head) units chunk by chunk; with S the
+// carry, g^|r-j| and the weights W of a chunk's rows:
 //
-//   P = (Q K^T) * g^|r-j| on the causal side      O  = P V + W_out Q S
-//   D = (W_kv K)^T V                               S <- g^n S + c D
+//   outputs  P = (Q K^T) * g^|r-j| on the causal side    O = P V + W_out (Q S)
+//            D = (W_kv K)^T V                             S <- g^n S + c D
+//   states   D and S only, with W_kv K in two (fp16) or three (bf16) 16-bit parts
+//            whose sum keeps all its bits: the memories that leave the operator
+//            are good to fp32, while the carry inside the outputs kernel, which is
+//            rounded to 16 bits before use, takes one part.
 //
-// Four matrix products on tcgen05 (M = 128), everything else on the way between
-// tensor memory and shared memory:
+// All products are tcgen05 (M = 128 steps or memory rows, sums in TMEM). 20 warps:
+//   warp 0      copies: Q, K, V, two stages of 128-byte-swizzled tiles
+//   warp 1      issues the products, one thread: P V, Q S, the next chunk's Q K^T,
+//               then (W_kv K)^T V
+//   warps 4-11  scores -> P (16 bits, back into TMEM as an A operand) and K -> W_kv K
+//               in place; two warps per 32 rows, half of the columns each
+//   warps 12-19 outputs; the carry in fp32 registers (row per lane, half of the
+//               columns), rounded into shared memory as the next chunk's operand
+// Registers move from the first three warpgroups to the last two (setmaxnreg).
 //
-//   warp 0     copies: Q (one buffer), K and V (two each), 128-byte swizzle
-//   warp 1     issues the products, one thread
-//   warps 2-5  scores (TMEM) -> P (16 bits, back into TMEM as an A operand);
-//              K -> W_kv K in place, and what rounding left of it into a second
-//              buffer, so that D is good to 2^-16 of its terms
-//   warps 6-9  outputs; the carry in fp32 registers (thread = row of S), rounded
-//              into shared memory as the next chunk's operand
-//
-// What bounds it: the bytes of q, k, v and o (one read, one write) while there
-// are enough (row, head) pairs for the SMs; per chunk of 128 x 128 heads that is
-// 128 KB or 5.6 thousand cycles of one SM's share of the copy bandwidth, against
-// about 2.6 thousand for the products and 2 thousand for either group of warps.
+// What bounds it: the bytes of q, k, v and o (one read, one write); a chunk of
+// 128-wide heads is 128 KB, 5.6 thousand cycles of one SM's share of the copy
+// bandwidth. Its four products are about 100 cycles per 128 x 128 x 16 step
+// (shared-memory reads of both operands bound them), 3.2 thousand in all, and the
+// loop scores -> P -> P V -> next scores about 3.7 thousand.
 #include <cuda.h>
 #include <math.h>
 
@@ -35,34 +40,33 @@ namespace mb {
 namespace {
 
 constexpr int kC = 128;  // steps per chunk: the M of one product
-constexpr int kTcThreads = 320;
+constexpr int kTcThreads = 640;
 constexpr int kBlockBytes = kC * 128;  // 64 columns x 128 steps of 16 bits
 constexpr int64_t kTcMinSteps = 16;    // below: the recurrent kernel
+constexpr int kGroup = 256;            // threads of each of the two worker groups
 
 struct TcArgs {
   mb_decay_attention_args a;
   AttnSplit split;
+  int64_t units;  // segments x B x H
   // whether a dimension's coordinate counts (0: the tensor is broadcast along it)
   int32_t q_b, q_h, k_b, k_h, v_b, v_h;
 };
 
 template <int DK, int DV>
-struct TcLayout {
+struct OutLayout {
   static constexpr int kQBytes = kC * DK * 2;
   static constexpr int kVBytes = kC * DV * 2;
-  static constexpr int kSBytes = DK * DV * 2;
-  static constexpr int kQ = 0;
-  static constexpr int kK = kQ + kQBytes;       // two stages
-  static constexpr int kLo = kK + 2 * kQBytes;  // rounding remainders of W_kv K
-  static constexpr int kV = kLo + kQBytes;      // two stages
+  static constexpr int kQ = 0;  // two stages each of Q, K and V
+  static constexpr int kK = kQ + 2 * kQBytes;
+  static constexpr int kV = kK + 2 * kQBytes;
   static constexpr int kS = kV + 2 * kVBytes;
-  static constexpr int kTables = kS + kSBytes;
-  static constexpr int kPow = kTables;                  // g^n, n = 0..128
-  static constexpr int kWeights = kPow + 132 * 4;       // weights of the scores by distance
-  static constexpr int kRowScale = kWeights + 256 * 4;  // fp16: 1 / scale of P's rows, two chunks
-  static constexpr int kMax = kRowScale + 2 * kC * 4;    // fp16: largest carry of each warp
-  static constexpr int kBars = kMax + 32;
-  static constexpr int kNumBars = 15;
+  static constexpr int kWeights = kS + DK * DV * 2;      // weights of the scores by distance
+  static constexpr int kRowScale = kWeights + 256 * 4;   // fp16: 1 / scale of P's rows, by stage
+  static constexpr int kRowTop = kRowScale + 2 * kC * 4;  // fp16: largest of the other half
+  static constexpr int kMax = kRowTop + kC * 4;           // fp16: largest values of each warp
+  static constexpr int kBars = kMax + 2 * 8 * 4;
+  static constexpr int kNumBars = 18;
   static constexpr size_t kSmem = kBars + kNumBars * 8 + 16;
   static_assert(kBars % 8 == 0 && kSmem <= 232448, "shared memory");
   // TMEM columns
@@ -70,8 +74,60 @@ struct TcLayout {
   static constexpr uint32_t kIntra = 128;
   static constexpr uint32_t kInter = kIntra + DV;
   static constexpr uint32_t kDelta = kInter + DV;
-  static constexpr uint32_t kTmemCols = 512;
 };
+
+template <int DK, int DV, int PARTS>
+struct StatesLayout {
+  static constexpr int kKBytes = kC * DK * 2;
+  static constexpr int kVBytes = kC * DV * 2;
+  static constexpr int kK = 0;  // two stages each
+  static constexpr int kLo = kK + 2 * kKBytes;  // the further parts of W_kv K
+  static constexpr int kV = kLo + (PARTS - 1) * kKBytes;
+  static constexpr int kBars = kV + 2 * kVBytes;
+  static constexpr int kNumBars = 10;
+  static constexpr size_t kSmem = kBars + kNumBars * 8 + 16;
+  static_assert(kSmem <= 232448, "shared memory");
+  static constexpr uint32_t kDelta = 0;
+};
+
+// One (segment, batch row, head): its valid steps [lo, end) and their chunks.
+struct Unit {
+  int b, h;
+  int64_t seg, lo, hi, end;
+  int chunks;
+  float log2g;
+};
+
+__device__ __forceinline__ Unit decode_unit(const TcArgs& args, int64_t unit) {
+  const mb_decay_attention_args& a = args.a;
+  Unit u;
+  u.h = static_cast<int>(unit % a.H);
+  u.b = static_cast<int>(unit / a.H % a.B);
+  u.seg = unit / a.H / a.B;
+  u.lo = u.seg * args.split.len;
+  u.hi = imin64(a.T, u.lo + args.split.len);
+  u.end = imin64(u.hi, attn_row_length(a.lengths, u.b, a.T));
+  u.chunks = u.end > u.lo ? static_cast<int>((u.end - u.lo + kC - 1) / kC) : 0;
+  u.log2g = log2f(a.decay[u.h]);
+  return u;
+}
+
+// First step of the unit's i-th chunk in processing order, and its valid steps.
+__device__ __forceinline__ int64_t chunk_t0(const Unit& u, int i, bool reverse) {
+  return u.lo + int64_t(reverse ? u.chunks - 1 - i : i) * kC;
+}
+__device__ __forceinline__ int chunk_steps(const Unit& u, int64_t t0) {
+  return static_cast<int>(imin64(kC, u.end - t0));
+}
+
+// Weight of row r (< n) of a chunk of n steps in the carry that leaves it, and of
+// the carry that enters it in row r's output.
+__device__ __forceinline__ float kv_weight(const Unit& u, int r, int n, bool reverse) {
+  return decay_pow(u.log2g, reverse ? r + 1 : n - 1 - r);
+}
+__device__ __forceinline__ float out_weight(const Unit& u, int r, int n, bool reverse) {
+  return decay_pow(u.log2g, reverse ? n - 1 - r : r + 1);
+}
 
 template <typename T>
 __device__ __forceinline__ uint32_t tc_idesc(int n, bool a_mn, bool b_mn) {
@@ -171,6 +227,8 @@ __device__ __forceinline__ float fp16_scale(float top) {
   return __uint_as_float(static_cast<uint32_t>(s) << 23);
 }
 
+// Barriers 1..: 1 the score warps, 2 the carry warps, 3.. the two score warps of
+// one TMEM lane quarter.
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -181,329 +239,417 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   if (lane == 0) mbar_arrive(bar);
 }
 
-template <typename T, int DK, int DV, bool STATES_ONLY>
-__global__ void __launch_bounds__(kTcThreads, 1)
-    attn_chunk_kernel(const __grid_constant__ CUtensorMap map_q,
-                      const __grid_constant__ CUtensorMap map_k,
-                      const __grid_constant__ CUtensorMap map_v,
-                      const __grid_constant__ TcArgs args) {
-  using L = TcLayout<DK, DV>;
-  constexpr bool kHalf = std::is_same<T, __half>::value;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  float* pow_t = reinterpret_cast<float*>(smem + L::kPow);
-  float* weights = reinterpret_cast<float*>(smem + L::kWeights);
-  float* row_scale = reinterpret_cast<float*>(smem + L::kRowScale);
-  float* warp_max = reinterpret_cast<float*>(smem + L::kMax);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
-  uint64_t* full_q = bars;
-  uint64_t* full_k = bars + 1;   // [2]
-  uint64_t* full_v = bars + 3;   // [2]
-  uint64_t* empty_q = bars + 5;
-  uint64_t* empty_kv = bars + 6;  // [2]
-  uint64_t* scores_done = bars + 8;
-  uint64_t* p_ready = bars + 9;
-  uint64_t* kw_ready = bars + 10;
-  uint64_t* out_done = bars + 11;
-  uint64_t* delta_done = bars + 12;
-  uint64_t* carry_ready = bars + 13;
-  uint64_t* drained = bars + 14;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
 
-  const mb_decay_attention_args& a = args.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int64_t u = blockIdx.x;
-  const int h = static_cast<int>(u % a.H);
-  u /= a.H;
-  const int b = static_cast<int>(u % a.B);
-  const int64_t seg = u / a.B;
-  const int64_t len = attn_row_length(a.lengths, b, a.T);
-  const int64_t lo = seg * args.split.len;
-  const int64_t hi = imin64(a.T, lo + args.split.len);
-  const int64_t end = imin64(hi, len);
-  const int chunks = end > lo ? static_cast<int>((end - lo + kC - 1) / kC) : 0;
-  const bool reverse = a.reverse != 0;
-  const float log2g = log2f(a.decay[h]);
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
 
-  auto chunk_t0 = [&](int i) {  // first step of the i-th chunk in processing order
-    return lo + int64_t(reverse ? chunks - 1 - i : i) * kC;
-  };
-  auto chunk_steps = [&](int64_t t0) { return static_cast<int>(imin64(kC, end - t0)); };
-
-  for (int i = threadIdx.x; i <= kC; i += kTcThreads) {
-    pow_t[i] = decay_pow(log2g, i);
-  }
-  // weights[128 + r - j]: scale * g^|r - j| of the causal side, 0 of the other
-  for (int i = threadIdx.x; i < 256; i += kTcThreads) {
-    const int d = reverse ? 128 - i : i - 128;
-    weights[i] = d >= 0 ? decay_pow(log2g, d) * (a.out_scale * a.kv_scale) : 0.0f;
-  }
-  if (threadIdx.x == 0) {
-    mbar_init(full_q, 1);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&full_k[s], 1);
-      mbar_init(&full_v[s], 1);
-      mbar_init(&empty_kv[s], 1);
-    }
-    mbar_init(empty_q, 1);
-    mbar_init(scores_done, 1);
-    mbar_init(p_ready, 4);
-    mbar_init(kw_ready, 4);
-    mbar_init(out_done, 2);  // the product's completion, and what its operand's makers wrote
-    mbar_init(delta_done, 1);
-    mbar_init(carry_ready, 4);
-    mbar_init(drained, 1);
-    fence_barrier_init();
-  }
+__device__ __forceinline__ uint32_t tmem_alloc(uint32_t* slot, int warp) {
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_addr(tmem_slot)),
-                 "r"(L::kTmemCols));
+                     smem_addr(slot)),
+                 "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  return *slot;
+}
 
-  if (warp == 0) {
-    if (lane == 0) {
-      const int qh = h * args.q_h, qb = b * args.q_b, kh = h * args.k_h, kb = b * args.k_b;
-      const int vh = h * args.v_h, vb = b * args.v_b;
-      int issued = 0;
-      for (int i = 0; i < chunks; ++i) {
-        const int s = i & 1;
-        const int t = static_cast<int>(chunk_t0(i));
-        if (i >= 2 && !mbar_wait_bounded(&empty_kv[s], ((i >> 1) - 1) & 1)) break;
-        mbar_arrive_expect_tx(&full_k[s], L::kQBytes);
-        for (int x = 0; x < DK / 64; ++x) {
-          tma_load_4d(smem + L::kK + s * L::kQBytes + x * kBlockBytes, &map_k, x * 64, t, kh, kb,
-                      &full_k[s]);
-        }
-        mbar_arrive_expect_tx(&full_v[s], L::kVBytes);
-        for (int x = 0; x < DV / 64; ++x) {
-          tma_load_4d(smem + L::kV + s * L::kVBytes + x * kBlockBytes, &map_v, x * 64, t, vh, vb,
-                      &full_v[s]);
-        }
-        issued = i + 1;
-        if constexpr (!STATES_ONLY) {
-          if (i >= 1 && !mbar_wait_bounded(empty_q, (i - 1) & 1)) break;
-          mbar_arrive_expect_tx(full_q, L::kQBytes);
+__device__ __forceinline__ void tmem_free(uint32_t tmem, int warp) {
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+// COLS values of one memory row (element c at p[c * stride], c < valid), zeros
+// where p is null or past `valid`.
+template <int COLS>
+__device__ __forceinline__ void load_memory_row(const float* p, int64_t stride, int64_t valid,
+                                                float (&S)[COLS]) {
+  if (p == nullptr || valid <= 0) {
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) S[c] = 0.0f;
+  } else if (stride == 1 && valid >= COLS && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+    for (int c = 0; c < COLS; c += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(p + c);
+      S[c] = x.x;
+      S[c + 1] = x.y;
+      S[c + 2] = x.z;
+      S[c + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) S[c] = c < valid ? p[c * stride] : 0.0f;
+  }
+}
+
+template <int COLS>
+__device__ __forceinline__ void store_memory_row(float* p, int64_t stride, int64_t valid,
+                                                 const float (&S)[COLS]) {
+  if (p == nullptr) return;
+  if (stride == 1 && valid >= COLS && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+    for (int c = 0; c < COLS; c += 4) {
+      *reinterpret_cast<float4*>(p + c) = make_float4(S[c], S[c + 1], S[c + 2], S[c + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+      if (c < valid) p[c * stride] = S[c];
+    }
+  }
+}
+
+// Values past the row's end may hold anything (0 * NaN must not reach a sum):
+// this thread's half of row r of a V tile becomes zero.
+template <int DV>
+__device__ __forceinline__ void zero_v_row(uint8_t* vs, int r, int half) {
+#pragma unroll
+  for (int q = 0; q < DV / 16; ++q) {
+    *reinterpret_cast<uint4*>(vs + piece_at(r, half * (DV / 16) + q, kC)) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Outputs
+// ---------------------------------------------------------------------------
+template <typename T, int DK, int DV>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    attn_out_kernel(const __grid_constant__ CUtensorMap map_q,
+                    const __grid_constant__ CUtensorMap map_k,
+                    const __grid_constant__ CUtensorMap map_v,
+                    const __grid_constant__ TcArgs args) {
+  using L = OutLayout<DK, DV>;
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  constexpr int kCols = DV / 2;  // memory and output columns per worker thread
+  extern __shared__ __align__(1024) uint8_t smem[];
+  float* weights = reinterpret_cast<float*>(smem + L::kWeights);
+  float* row_scale = reinterpret_cast<float*>(smem + L::kRowScale);
+  float* row_top = reinterpret_cast<float*>(smem + L::kRowTop);
+  float* warp_max = reinterpret_cast<float*>(smem + L::kMax);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* full_q = bars;            // [2]
+  uint64_t* full_k = bars + 2;        // [2]
+  uint64_t* full_v = bars + 4;        // [2]
+  uint64_t* empty = bars + 6;         // [2] a stage's Q, K and V
+  uint64_t* scores_done = bars + 8;
+  uint64_t* p_ready = bars + 9;
+  uint64_t* pv_done = bars + 10;
+  uint64_t* out_done = bars + 11;
+  uint64_t* out_read = bars + 12;
+  uint64_t* kw_ready = bars + 13;
+  uint64_t* delta_done = bars + 14;
+  uint64_t* carry_ready = bars + 15;
+  uint64_t* drained = bars + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
+
+  const mb_decay_attention_args& a = args.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool reverse = a.reverse != 0;
+  // whether units start from a memory; without one their first chunk has no Q S
+  const bool carry_in = args.split.segments > 1 || a.first.data != nullptr;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&full_q[s], 1);
+      mbar_init(&full_k[s], 1);
+      mbar_init(&full_v[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(scores_done, 1);
+    mbar_init(p_ready, 8);
+    mbar_init(pv_done, 1);
+    mbar_init(out_done, 2);  // the products' completion, and what their operands' makers wrote
+    mbar_init(out_read, 8);
+    mbar_init(kw_ready, 8);
+    mbar_init(delta_done, 1);
+    mbar_init(carry_ready, 8);
+    mbar_init(drained, 1);
+    fence_barrier_init();
+  }
+  const uint32_t tmem = tmem_alloc(tmem_slot, warp);
+
+  // Parities: `it` counts chunks over all of the CTA's units (stage it & 1), `hand`
+  // the chunks whose carry goes on (all but each unit's last), `cin` the chunks
+  // that a carry enters. All roles count alike.
+  if (warp < 4) {
+    reg_dec<56>();
+    if (warp == 0 && lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
+        const Unit u = decode_unit(args, unit);
+        const int qh = u.h * args.q_h, qb = u.b * args.q_b, kh = u.h * args.k_h;
+        const int kb = u.b * args.k_b, vh = u.h * args.v_h, vb = u.b * args.v_b;
+        for (int i = 0; i < u.chunks; ++i, ++it) {
+          const int s = it & 1;
+          const int t = static_cast<int>(chunk_t0(u, i, reverse));
+          if (it >= 2 && !mbar_wait_bounded(&empty[s], ((it >> 1) - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full_q[s], L::kQBytes);
+          mbar_arrive_expect_tx(&full_k[s], L::kQBytes);
+          mbar_arrive_expect_tx(&full_v[s], L::kVBytes);
+#pragma unroll
           for (int x = 0; x < DK / 64; ++x) {
-            tma_load_4d(smem + L::kQ + x * kBlockBytes, &map_q, x * 64, t, qh, qb, full_q);
+            tma_load_4d(smem + L::kQ + s * L::kQBytes + x * kBlockBytes, &map_q, x * 64, t, qh, qb,
+                        &full_q[s]);
+            tma_load_4d(smem + L::kK + s * L::kQBytes + x * kBlockBytes, &map_k, x * 64, t, kh, kb,
+                        &full_k[s]);
+          }
+#pragma unroll
+          for (int x = 0; x < DV / 64; ++x) {
+            tma_load_4d(smem + L::kV + s * L::kVBytes + x * kBlockBytes, &map_v, x * 64, t, vh, vb,
+                        &full_v[s]);
           }
         }
       }
       // every issued copy has landed before the CTA can retire
-      for (int i = issued > 2 ? issued - 2 : 0; i < issued; ++i) {
-        (void)mbar_wait_bounded(&full_k[i & 1], (i >> 1) & 1);
-        (void)mbar_wait_bounded(&full_v[i & 1], (i >> 1) & 1);
+      for (uint32_t j = it > 2 ? it - 2 : 0; j < it; ++j) {
+        (void)mbar_wait_bounded(&full_q[j & 1], (j >> 1) & 1);
+        (void)mbar_wait_bounded(&full_k[j & 1], (j >> 1) & 1);
+        (void)mbar_wait_bounded(&full_v[j & 1], (j >> 1) & 1);
       }
-      if (!STATES_ONLY && issued == chunks && chunks > 0) {
-        (void)mbar_wait_bounded(full_q, (chunks - 1) & 1);
-      }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
+    } else if (warp == 1 && lane == 0) {
       const uint32_t i_scores = tc_idesc<T>(kC, false, false);
       const uint32_t i_out = tc_idesc<T>(DV, false, true);
       const uint32_t i_delta = tc_idesc<T>(DV, true, true);
       const uint32_t sq = smem_addr(smem + L::kQ), sk = smem_addr(smem + L::kK);
-      const uint32_t slo = smem_addr(smem + L::kLo), sv = smem_addr(smem + L::kV);
-      const uint32_t ss = smem_addr(smem + L::kS);
-      auto scores = [&](int i) {
-        if (!mbar_wait_bounded(full_q, i & 1) ||
-            !mbar_wait_bounded(&full_k[i & 1], (i >> 1) & 1)) {
+      const uint32_t sv = smem_addr(smem + L::kV), ss = smem_addr(smem + L::kS);
+      uint32_t it = 0, hand = 0, cin = 0;
+      bool ok = true;
+      auto scores = [&](uint32_t j) {
+        const int s = j & 1;
+        if (!mbar_wait_bounded(&full_q[s], (j >> 1) & 1) ||
+            !mbar_wait_bounded(&full_k[s], (j >> 1) & 1)) {
           return false;
         }
         tc_fence_after();
-        const uint32_t k0 = sk + (i & 1) * L::kQBytes;
 #pragma unroll
         for (int k = 0; k < DK / 16; ++k) {
-          const uint32_t at = (k >> 2) * kBlockBytes + (k & 3) * 32;
-          mma_f16(tmem + L::kScores, sw128_kmajor_desc(sq + at), sw128_kmajor_desc(k0 + at),
+          const uint32_t at = s * L::kQBytes + (k >> 2) * kBlockBytes + (k & 3) * 32;
+          mma_f16(tmem + L::kScores, sw128_kmajor_desc(sq + at), sw128_kmajor_desc(sk + at),
                   i_scores, k != 0);
         }
         mma_commit(scores_done);
         return true;
       };
-      bool ok = true;
-      if (!STATES_ONLY && chunks > 0) ok = scores(0);
-      for (int i = 0; i < chunks && ok; ++i) {
-        const int s = i & 1;
-        const uint32_t v0 = sv + s * L::kVBytes;
-        // the carry's operand is written, and what the accumulators held has been read
-        if (!mbar_wait_bounded(carry_ready, i & 1)) break;
-        tc_fence_after();
-        if constexpr (!STATES_ONLY) {
-#pragma unroll
-          for (int k = 0; k < DK / 16; ++k) {
-            mma_f16(tmem + L::kInter,
-                    sw128_kmajor_desc(sq + (k >> 2) * kBlockBytes + (k & 3) * 32),
-                    mn_desc(ss + k * 2048, DK * 128), i_out, k != 0);
-          }
-          mma_commit(empty_q);
-          if (!mbar_wait_bounded(p_ready, i & 1)) break;
-          if (!mbar_wait_bounded(&full_v[s], (i >> 1) & 1)) break;
+      // the next chunk's scores are issued a chunk ahead, across units
+      int64_t unit = blockIdx.x;
+      auto next_unit = [&](int64_t from) {
+        int64_t x = from;
+        while (x < args.units && decode_unit(args, x).chunks == 0) x += gridDim.x;
+        return x;
+      };
+      unit = next_unit(unit);
+      if (unit < args.units) ok = scores(0);
+      while (unit < args.units && ok) {
+        const Unit u = decode_unit(args, unit);
+        const int64_t following = next_unit(unit + gridDim.x);
+        for (int i = 0; i < u.chunks; ++i, ++it) {
+          const int s = it & 1;
+          const uint32_t v0 = sv + s * L::kVBytes;
+          const bool last = i + 1 == u.chunks;
+          ok = false;
+          // P is written, and the last chunk's outputs have been read
+          if (!mbar_wait_bounded(p_ready, it & 1)) break;
+          if (it >= 1 && !mbar_wait_bounded(out_read, (it - 1) & 1)) break;
+          if (!mbar_wait_bounded(&full_v[s], (it >> 1) & 1)) break;
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < kC / 16; ++k) {
             mma_f16_ts(tmem + L::kIntra, tmem + L::kScores + k * 8,
                        mn_desc(v0 + k * 2048, kBlockBytes), i_out, k != 0);
           }
+          mma_commit(pv_done);
+          if (i > 0 || carry_in) {
+            if (!mbar_wait_bounded(carry_ready, cin & 1)) break;
+            ++cin;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < DK / 16; ++k) {
+              mma_f16(tmem + L::kInter,
+                      sw128_kmajor_desc(sq + s * L::kQBytes + (k >> 2) * kBlockBytes + (k & 3) * 32),
+                      mn_desc(ss + k * 2048, DK * 128), i_out, k != 0);
+            }
+          }
           mma_commit(out_done);
           mbar_arrive(out_done);
-          if (i + 1 < chunks) {
+          if (!last || following < args.units) {
             // the next scores overwrite P: its product has to be complete
-            if (!mbar_wait_bounded(out_done, i & 1)) break;
-            if (!scores(i + 1)) break;
+            if (!mbar_wait_bounded(pv_done, it & 1)) break;
+            if (!scores(it + 1)) break;
           }
-        } else {
-          if (!mbar_wait_bounded(&full_v[s], (i >> 1) & 1)) break;
-        }
-        if (!mbar_wait_bounded(kw_ready, i & 1)) break;
-        tc_fence_after();
-        const uint32_t k0 = sk + s * L::kQBytes;
+          if (!last) {
+            if (!mbar_wait_bounded(kw_ready, hand & 1)) break;
+            ++hand;
+            tc_fence_after();
+            const uint32_t k0 = sk + s * L::kQBytes;
 #pragma unroll
-        for (int k = 0; k < kC / 16; ++k) {
-          mma_f16(tmem + L::kDelta, mn_desc(slo + k * 2048, kBlockBytes),
-                  mn_desc(v0 + k * 2048, kBlockBytes), i_delta, k != 0);
+            for (int k = 0; k < kC / 16; ++k) {
+              mma_f16(tmem + L::kDelta, mn_desc(k0 + k * 2048, kBlockBytes),
+                      mn_desc(v0 + k * 2048, kBlockBytes), i_delta, k != 0);
+            }
+            mma_commit(delta_done);
+          }
+          mma_commit(&empty[s]);
+          ok = true;
         }
-#pragma unroll
-        for (int k = 0; k < kC / 16; ++k) {
-          mma_f16(tmem + L::kDelta, mn_desc(k0 + k * 2048, kBlockBytes),
-                  mn_desc(v0 + k * 2048, kBlockBytes), i_delta, 1u);
-        }
-        mma_commit(delta_done);
-        mma_commit(&empty_kv[s]);
+        unit = following;
       }
       // all products and commits are complete before TMEM is released
       mma_commit(drained);
       (void)mbar_wait_bounded(drained, 0);
     }
-  } else if (warp < 6) {
-    const int quarter = warp & 3;
+  } else if (warp < 12) {
+    reg_dec<80>();
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
     const int r = quarter * 32 + lane;
     const uint32_t t_scores = tmem + L::kScores + (uint32_t(quarter * 32) << 16);
     const float* w_row = weights + 128 + r;  // w_row[-j]: weight of step j for this row
-    for (int i = 0; i < chunks; ++i) {
-      const int s = i & 1;
-      const int n = chunk_steps(chunk_t0(i));
-      uint8_t* ks = smem + L::kK + s * L::kQBytes;
-      uint8_t* vs = smem + L::kV + s * L::kVBytes;
-      if (!mbar_wait_bounded(&full_k[s], (i >> 1) & 1)) break;
-      if (n < kC) {
-        // values past the row's end may hold anything: 0 * NaN must not reach a sum
-        if (!mbar_wait_bounded(&full_v[s], (i >> 1) & 1)) break;
-        if (r >= n) {
-#pragma unroll
-          for (int q = 0; q < DV / 8; ++q) {
-            *reinterpret_cast<uint4*>(vs + piece_at(r, q, kC)) = make_uint4(0, 0, 0, 0);
-          }
-        }
-        fence_proxy_async_smem();
+    uint32_t it = 0;
+    bool ok = true;
+    for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
+      const Unit u = decode_unit(args, unit);
+      if (u.chunks == 0) continue;
+      // weights[128 + r - j]: scale * g^|r - j| of the causal side, 0 of the other
+      bar_sync(1, kGroup);  // the last unit's have been read
+      {
+        const int x = threadIdx.x - 128;
+        const int d = reverse ? 128 - x : x - 128;
+        weights[x] = d >= 0 ? decay_pow(u.log2g, d) * (a.out_scale * a.kv_scale) : 0.0f;
       }
-      if constexpr (!STATES_ONLY) {
-        if (!mbar_wait_bounded(scores_done, i & 1)) break;
+      bar_sync(1, kGroup);
+      for (int i = 0; i < u.chunks; ++i, ++it) {
+        const int s = it & 1;
+        const int n = chunk_steps(u, chunk_t0(u, i, reverse));
+        uint8_t* ks = smem + L::kK + s * L::kQBytes;
+        ok = false;
+        if (!mbar_wait_bounded(&full_k[s], (it >> 1) & 1)) break;
+        if (n < kC) {
+          if (!mbar_wait_bounded(&full_v[s], (it >> 1) & 1)) break;
+          if (r >= n) zero_v_row<DV>(smem + L::kV + s * L::kVBytes, r, half);
+          fence_proxy_async_smem();
+        }
+        if (!mbar_wait_bounded(scores_done, it & 1)) break;
         tc_fence_after();
-        // column blocks wholly on the other side of the diagonal are zero
-        auto empty = [&](int jb) { return reverse ? jb < quarter : jb > quarter; };
-        // in reverse, steps past the row's end lie on the causal side
+        // column blocks half and half + 2; those wholly on the other side of the
+        // diagonal are zero, and in reverse steps past the row's end are, too
+        auto blank = [&](int jb) { return reverse ? jb < quarter : jb > quarter; };
         const int last = reverse ? n : kC;
         float scale = 1.0f;
         if constexpr (kHalf) {
           // fp16: P's rows are brought to a common magnitude by a power of two
           float top = 0.0f;
 #pragma unroll
-          for (int jb = 0; jb < 4; ++jb) {
-            if (empty(jb)) continue;
-            uint32_t x[32];
-            tmem_ld32_issue(t_scores + jb * 32, x);
-            tmem_wait_ld();
+          for (int x = 0; x < 2; ++x) {
+            const int jb = half + 2 * x;
+            if (blank(jb)) continue;
+            const float* wj = w_row - jb * 32;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float w = fabsf(__uint_as_float(x[j]) * w_row[-(jb * 32 + j)]);
-              top = fmaxf(top, jb * 32 + j < last ? w : 0.0f);  // drops a NaN
+            for (int y = 0; y < 32; y += 16) {
+              uint32_t v[16];
+              tmem_ld16_issue(t_scores + jb * 32 + y, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const float w = fabsf(__uint_as_float(v[j]) * wj[-(y + j)]);
+                top = fmaxf(top, jb * 32 + y + j < last ? w : 0.0f);  // drops a NaN
+              }
             }
           }
-          scale = fp16_scale(top);
-          row_scale[s * kC + r] = 1.0f / scale;
+          (half == 0 ? row_scale + s * kC : row_top)[r] = top;
+          bar_sync(3 + quarter, 64);
+          scale = fp16_scale(fmaxf(row_scale[s * kC + r], row_top[r]));
         }
+        uint32_t p[2][16];
 #pragma unroll
-        for (int jb = 0; jb < 4; ++jb) {
-          uint32_t p[16];
-          if (empty(jb)) {
+        for (int x = 0; x < 2; ++x) {
+          const int jb = half + 2 * x;
+          if (blank(jb)) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) p[j] = 0;
+            for (int j = 0; j < 16; ++j) p[x][j] = 0;
           } else {
-            uint32_t x[32];
-            tmem_ld32_issue(t_scores + jb * 32, x);
-            tmem_wait_ld();
+            const float* wj = w_row - jb * 32;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              // a select: what a zero weight hides may be infinite or NaN
-              const float w = jb * 32 + j < last ? w_row[-(jb * 32 + j)] : 0.0f;
-              const float v = __uint_as_float(x[j]) * (kHalf ? w * scale : w);
-              x[j] = __float_as_uint(w != 0.0f ? v : 0.0f);
-            }
+            for (int y = 0; y < 32; y += 16) {
+              uint32_t v[16];
+              tmem_ld16_issue(t_scores + jb * 32 + y, v);
+              float w[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              p[j] = pack2<T>(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+              for (int j = 0; j < 16; ++j) {
+                w[j] = jb * 32 + y + j < last ? wj[-(y + j)] : 0.0f;
+              }
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; j += 2) {
+                // selects: what a zero weight hides may be infinite or NaN
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const float m = __uint_as_float(v[j + e]) * (kHalf ? w[j + e] * scale : w[j + e]);
+                  f[e] = w[j + e] != 0.0f ? m : 0.0f;
+                }
+                p[x][(y + j) / 2] = pack2<T>(f[0], f[1]);
+              }
             }
           }
-          // overwrites scores of blocks that this thread has read
-          tmem_st16(t_scores + jb * 16, p);
+        }
+        bar_sync(3 + quarter, 64);  // both warps have read the scores that P overwrites
+#pragma unroll
+        for (int x = 0; x < 2; ++x) tmem_st16(t_scores + (half + 2 * x) * 16, p[x]);
+        if constexpr (kHalf) {
+          // for the output warps, which have read this stage's last ones (P V of
+          // the chunk between waited for that)
+          if (half == 0) row_scale[s * kC + r] = 1.0f / scale;
         }
         tmem_wait_st();
         tc_fence_before();
         warp_arrive(p_ready, lane);
-      }
-      // the remainders' buffer is free once the last chunk's D is complete
-      if (i >= 1 && !mbar_wait_bounded(delta_done, (i - 1) & 1)) break;
-      const float w = r < n ? pow_t[reverse ? r + 1 : n - 1 - r] : 0.0f;
+        if (i + 1 < u.chunks) {
+          // K <- W_kv K for the carry; the scores that read K are complete
+          const float w = r < n ? kv_weight(u, r, n, reverse) : 0.0f;
 #pragma unroll
-      for (int q = 0; q < DK / 8; ++q) {
-        const int at = piece_at(r, q, kC);
-        const uint4 x = *reinterpret_cast<const uint4*>(ks + at);
-        const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-        uint32_t hi16[4], lo16[4];
+          for (int q = 0; q < DK / 16; ++q) {
+            uint4* at = reinterpret_cast<uint4*>(ks + piece_at(r, half * (DK / 16) + q, kC));
+            const uint4 x = *at;
+            const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+            uint32_t y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = unpack2<T>(in[e]);
-          const float f0 = r < n ? f.x * w : 0.0f, f1 = r < n ? f.y * w : 0.0f;
-          hi16[e] = pack2<T>(f0, f1);
-          const float2 back = unpack2<T>(hi16[e]);
-          lo16[e] = pack2<T>(f0 - back.x, f1 - back.y);
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = unpack2<T>(in[e]);
+              y[e] = r < n ? pack2<T>(f.x * w, f.y * w) : 0u;
+            }
+            *at = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+          fence_proxy_async_smem();
+          warp_arrive(kw_ready, lane);
         }
-        *reinterpret_cast<uint4*>(ks + at) = make_uint4(hi16[0], hi16[1], hi16[2], hi16[3]);
-        *reinterpret_cast<uint4*>(smem + L::kLo + at) =
-            make_uint4(lo16[0], lo16[1], lo16[2], lo16[3]);
+        ok = true;
       }
-      fence_proxy_async_smem();
-      warp_arrive(kw_ready, lane);
     }
   } else {
-    const int quarter = warp & 3;
+    reg_inc<128>();
+    const int quarter = warp & 3, half = (warp - 12) >> 2;
     const int r = quarter * 32 + lane;  // row of the carry, and step of a chunk
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    const bool row_ok = r < a.Dk;
+    const int col0 = half * kCols;
     const bool holds = quarter * 32 < DK;  // warps past DK hold no carry (uniform)
-    float S[DV];
-    {
-      const float* from = nullptr;
-      int64_t sc = 1;
-      if (!STATES_ONLY && row_ok) {
-        if (args.split.segments > 1) {
-          from = args.split.states + (((seg * a.B + b) * a.H + h) * a.Dk + r) * a.Dv;
-        } else if (a.first.data != nullptr) {
-          from = a.first.data + b * a.first.stride_b + h * a.first.stride_h +
-                 r * a.first.stride_row;
-          sc = a.first.stride_col;
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < DV; ++c) S[c] = from != nullptr && c < a.Dv ? from[c * sc] : 0.0f;
-    }
+    float S[kCols];
     float inv_s = 1.0f;  // fp16: 1 / scale of the carry's operand
+    uint32_t put = 0;
     // the carry, rounded, as the B operand of the next chunk (rows of S, MN-major)
     auto put_carry = [&]() {
       float scale = 1.0f;
@@ -511,52 +657,79 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         float top = 0.0f;
         if (holds) {
 #pragma unroll
-          for (int c = 0; c < DV; ++c) top = fmaxf(top, fabsf(S[c]));
+          for (int c = 0; c < kCols; ++c) top = fmaxf(top, fabsf(S[c]));
 #pragma unroll
           for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         }
-        bar_sync(1, 128);  // the last maxima have been read
-        if (lane == 0) warp_max[quarter] = top;
-        bar_sync(1, 128);
-        top = fmaxf(fmaxf(warp_max[0], warp_max[1]), fmaxf(warp_max[2], warp_max[3]));
+        float* at = warp_max + (put & 1) * 8;
+        ++put;
+        if (lane == 0) at[warp - 12] = top;
+        bar_sync(2, kGroup);
+        top = at[0];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) top = fmaxf(top, at[w]);
         scale = fp16_scale(top);
         inv_s = 1.0f / scale;
       }
       if (holds) {
 #pragma unroll
-        for (int q = 0; q < DV / 8; ++q) {
+        for (int q = 0; q < kCols / 8; ++q) {
           uint32_t x[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             x[e] = pack2<T>(S[8 * q + 2 * e] * scale, S[8 * q + 2 * e + 1] * scale);
           }
-          *reinterpret_cast<uint4*>(smem + L::kS + piece_at(r, q, DK)) =
+          *reinterpret_cast<uint4*>(smem + L::kS + piece_at(r, col0 / 8 + q, DK)) =
               make_uint4(x[0], x[1], x[2], x[3]);
         }
       }
       fence_proxy_async_smem();
-    };
-    if (chunks > 0) {
-      if constexpr (!STATES_ONLY) put_carry();
+      tc_fence_before();
       warp_arrive(carry_ready, lane);
-    }
-    T* o = static_cast<T*>(a.o.data) + b * a.o.stride_b + h * a.o.stride_h;
-    for (int i = 0; i < chunks; ++i) {
-      const int64_t t0 = chunk_t0(i);
-      const int n = chunk_steps(t0);
-      if constexpr (!STATES_ONLY) {
-        if (!mbar_wait_bounded(out_done, i & 1)) break;
+    };
+    uint32_t it = 0, hand = 0;
+    bool ok = true;
+    for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
+      const Unit u = decode_unit(args, unit);
+      T* o = static_cast<T*>(a.o.data) + u.b * a.o.stride_b + u.h * a.o.stride_h;
+      if (u.chunks > 0) {
+        const float* from = nullptr;
+        int64_t sc = 1;
+        if (r < a.Dk) {
+          if (args.split.segments > 1) {
+            from = args.split.states + (((u.seg * a.B + u.b) * a.H + u.h) * a.Dk + r) * a.Dv + col0;
+          } else if (a.first.data != nullptr) {
+            sc = a.first.stride_col;
+            from = a.first.data + u.b * a.first.stride_b + u.h * a.first.stride_h +
+                   r * a.first.stride_row + col0 * sc;
+          }
+        }
+        load_memory_row<kCols>(from, sc, a.Dv - col0, S);
+        // the last unit's operand has been read: its outputs were complete
+        if (carry_in) put_carry();
+      }
+      for (int i = 0; i < u.chunks; ++i, ++it) {
+        const int64_t t0 = chunk_t0(u, i, reverse);
+        const int n = chunk_steps(u, t0);
+        ok = false;
+        if (!mbar_wait_bounded(out_done, it & 1)) break;
         tc_fence_after();
-        const float w_in = kHalf ? row_scale[(i & 1) * kC + r] : 1.0f;
+        const float w_in = kHalf ? row_scale[(it & 1) * kC + r] : 1.0f;
+        const bool inter = i > 0 || carry_in;
         const float w_out =
-            r < n ? pow_t[reverse ? n - 1 - r : r + 1] * a.out_scale * inv_s : 0.0f;
-        const bool store = t0 + r < hi;  // steps past the row's length get zeros
-        T* row = o + (t0 + r) * a.o.stride_t;
+            r < n ? out_weight(u, r, n, reverse) * (a.out_scale * inv_s) : 0.0f;
+        const bool store = t0 + r < u.hi;  // steps past the row's length get zeros
+        T* row = o + (t0 + r) * a.o.stride_t + col0;
 #pragma unroll
-        for (int c0 = 0; c0 < DV; c0 += 16) {
+        for (int c0 = 0; c0 < kCols; c0 += 16) {
           uint32_t x[16], y[16];
-          tmem_ld16_issue(tmem + L::kIntra + lanes + c0, x);
-          tmem_ld16_issue(tmem + L::kInter + lanes + c0, y);
+          tmem_ld16_issue(tmem + L::kIntra + lanes + col0 + c0, x);
+          if (inter) {
+            tmem_ld16_issue(tmem + L::kInter + lanes + col0 + c0, y);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) y[j] = 0;
+          }
           tmem_wait_ld();
           uint32_t p[8];
 #pragma unroll
@@ -569,67 +742,269 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             p[j] = r < n ? pack2<T>(v[0], v[1]) : 0u;
           }
-          if (store && c0 < a.Dv) {
+          if (store && col0 + c0 < a.Dv) {
             *reinterpret_cast<uint4*>(row + c0) = make_uint4(p[0], p[1], p[2], p[3]);
-            if (c0 + 8 < a.Dv) {
+            if (col0 + c0 + 8 < a.Dv) {
               *reinterpret_cast<uint4*>(row + c0 + 8) = make_uint4(p[4], p[5], p[6], p[7]);
             }
           }
         }
-      }
-      if (!mbar_wait_bounded(delta_done, i & 1)) break;
-      tc_fence_after();
-      if (holds) {
-        const float gn = pow_t[n];
-#pragma unroll
-        for (int c0 = 0; c0 < DV; c0 += 32) {
-          uint32_t x[32];
-          tmem_ld32_issue(tmem + L::kDelta + lanes + c0, x);
-          tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            S[c0 + j] = fmaf(gn, S[c0 + j], a.kv_scale * __uint_as_float(x[j]));
-          }
-        }
-      }
-      if (i + 1 < chunks) {
-        if constexpr (!STATES_ONLY) put_carry();
         tc_fence_before();
-        warp_arrive(carry_ready, lane);
+        warp_arrive(out_read, lane);
+        if (i + 1 < u.chunks) {
+          if (!mbar_wait_bounded(delta_done, hand & 1)) break;
+          ++hand;
+          tc_fence_after();
+          if (holds) {
+            const float gn = decay_pow(u.log2g, n);
+#pragma unroll
+            for (int c0 = 0; c0 < kCols; c0 += 16) {
+              uint32_t x[16];
+              tmem_ld16_issue(tmem + L::kDelta + lanes + col0 + c0, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                S[c0 + j] = fmaf(gn, S[c0 + j], a.kv_scale * __uint_as_float(x[j]));
+              }
+            }
+          }
+          put_carry();
+        }
+        ok = true;
       }
-    }
-    if (!STATES_ONLY) {  // whole chunks past the row's length: zeros
-      for (int64_t t = lo + int64_t(chunks) * kC + r; t < hi; t += kC) {
+      // whole chunks past the row's length: zeros
+      for (int64_t t = u.lo + int64_t(u.chunks) * kC + r; t < u.hi; t += kC) {
         T* row = o + t * a.o.stride_t;
-        for (int c = 0; c < a.Dv; c += 8) {
+        for (int64_t c = col0; c < imin64(a.Dv, col0 + kCols); c += 8) {
           *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
         }
       }
     }
-    if (row_ok) {
-      float* to = nullptr;
-      int64_t sc = 1;
-      if (STATES_ONLY) {
-        to = args.split.states + (((seg * a.B + b) * a.H + h) * a.Dk + r) * a.Dv;
-      } else if (args.split.segments == 1 && a.last.data != nullptr) {
-        to = a.last.data + b * a.last.stride_b + h * a.last.stride_h + r * a.last.stride_row;
-        sc = a.last.stride_col;
-      }
-      if (to != nullptr) {
+  }
+  tmem_free(tmem, warp);
+}
+
+// ---------------------------------------------------------------------------
+// States: every unit's final memory (one segment: from `first` to `last`; more:
+// each segment's own, from zero, to the workspace)
+// ---------------------------------------------------------------------------
+template <typename T, int DK, int DV>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    attn_states_kernel(const __grid_constant__ CUtensorMap map_k,
+                       const __grid_constant__ CUtensorMap map_v,
+                       const __grid_constant__ TcArgs args) {
+  constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
+  using L = StatesLayout<DK, DV, PARTS>;
+  constexpr int kCols = DV / 2;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* full_k = bars;      // [2]
+  uint64_t* full_v = bars + 2;  // [2]
+  uint64_t* empty = bars + 4;   // [2]
+  uint64_t* kw_ready = bars + 6;
+  uint64_t* delta_done = bars + 7;
+  uint64_t* delta_read = bars + 8;
+  uint64_t* drained = bars + 9;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
+
+  const mb_decay_attention_args& a = args.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool reverse = a.reverse != 0;
+  const bool whole = args.split.segments == 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&full_k[s], 1);
+      mbar_init(&full_v[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(kw_ready, 8);
+    mbar_init(delta_done, 1);
+    mbar_init(delta_read, 8);
+    mbar_init(drained, 1);
+    fence_barrier_init();
+  }
+  const uint32_t tmem = tmem_alloc(tmem_slot, warp);
+
+  if (warp < 4) {
+    reg_dec<56>();
+    if (warp == 0 && lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
+        const Unit u = decode_unit(args, unit);
+        const int kh = u.h * args.k_h, kb = u.b * args.k_b, vh = u.h * args.v_h,
+                  vb = u.b * args.v_b;
+        for (int i = 0; i < u.chunks; ++i, ++it) {
+          const int s = it & 1;
+          const int t = static_cast<int>(chunk_t0(u, i, reverse));
+          if (it >= 2 && !mbar_wait_bounded(&empty[s], ((it >> 1) - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full_k[s], L::kKBytes);
+          mbar_arrive_expect_tx(&full_v[s], L::kVBytes);
 #pragma unroll
-        for (int c = 0; c < DV; ++c) {
-          if (c < a.Dv) to[c * sc] = S[c];
+          for (int x = 0; x < DK / 64; ++x) {
+            tma_load_4d(smem + L::kK + s * L::kKBytes + x * kBlockBytes, &map_k, x * 64, t, kh, kb,
+                        &full_k[s]);
+          }
+#pragma unroll
+          for (int x = 0; x < DV / 64; ++x) {
+            tma_load_4d(smem + L::kV + s * L::kVBytes + x * kBlockBytes, &map_v, x * 64, t, vh, vb,
+                        &full_v[s]);
+          }
         }
       }
+      for (uint32_t j = it > 2 ? it - 2 : 0; j < it; ++j) {
+        (void)mbar_wait_bounded(&full_k[j & 1], (j >> 1) & 1);
+        (void)mbar_wait_bounded(&full_v[j & 1], (j >> 1) & 1);
+      }
+    } else if (warp == 1 && lane == 0) {
+      const uint32_t i_delta = tc_idesc<T>(DV, true, true);
+      const uint32_t sk = smem_addr(smem + L::kK), slo = smem_addr(smem + L::kLo);
+      const uint32_t sv = smem_addr(smem + L::kV);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
+        const Unit u = decode_unit(args, unit);
+        for (int i = 0; i < u.chunks; ++i, ++it) {
+          const int s = it & 1;
+          ok = false;
+          if (!mbar_wait_bounded(kw_ready, it & 1)) break;
+          if (!mbar_wait_bounded(&full_v[s], (it >> 1) & 1)) break;
+          if (it >= 1 && !mbar_wait_bounded(delta_read, (it - 1) & 1)) break;
+          tc_fence_after();
+          const uint32_t v0 = sv + s * L::kVBytes;
+          // the smallest parts first
+#pragma unroll
+          for (int part = PARTS - 1; part >= 0; --part) {
+            const uint32_t k0 =
+                part == 0 ? sk + s * L::kKBytes : slo + (part - 1) * L::kKBytes;
+#pragma unroll
+            for (int k = 0; k < kC / 16; ++k) {
+              mma_f16(tmem + L::kDelta, mn_desc(k0 + k * 2048, kBlockBytes),
+                      mn_desc(v0 + k * 2048, kBlockBytes), i_delta,
+                      (part != PARTS - 1 || k != 0) ? 1u : 0u);
+            }
+          }
+          mma_commit(delta_done);
+          mma_commit(&empty[s]);
+          ok = true;
+        }
+      }
+      mma_commit(drained);
+      (void)mbar_wait_bounded(drained, 0);
+    }
+  } else if (warp < 12) {
+    reg_dec<80>();
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const int r = quarter * 32 + lane;
+    uint32_t it = 0;
+    bool ok = true;
+    for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
+      const Unit u = decode_unit(args, unit);
+      for (int i = 0; i < u.chunks; ++i, ++it) {
+        const int s = it & 1;
+        const int n = chunk_steps(u, chunk_t0(u, i, reverse));
+        uint8_t* ks = smem + L::kK + s * L::kKBytes;
+        ok = false;
+        if (!mbar_wait_bounded(&full_k[s], (it >> 1) & 1)) break;
+        if (n < kC) {
+          if (!mbar_wait_bounded(&full_v[s], (it >> 1) & 1)) break;
+          if (r >= n) zero_v_row<DV>(smem + L::kV + s * L::kVBytes, r, half);
+        }
+        // the further parts' buffers are free once the last chunk's D is complete
+        if (it >= 1 && !mbar_wait_bounded(delta_done, (it - 1) & 1)) break;
+        const float w = r < n ? kv_weight(u, r, n, reverse) : 0.0f;
+#pragma unroll
+        for (int q = 0; q < DK / 16; ++q) {
+          const int at = piece_at(r, half * (DK / 16) + q, kC);
+          const uint4 x = *reinterpret_cast<const uint4*>(ks + at);
+          const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 g = unpack2<T>(in[e]);
+            f[2 * e] = r < n ? g.x * w : 0.0f;
+            f[2 * e + 1] = r < n ? g.y * w : 0.0f;
+          }
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) {
+            uint32_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[e] = pack2<T>(f[2 * e], f[2 * e + 1]);
+              const float2 back = unpack2<T>(y[e]);
+              f[2 * e] -= back.x;
+              f[2 * e + 1] -= back.y;
+            }
+            uint8_t* to = part == 0 ? ks : smem + L::kLo + (part - 1) * L::kKBytes;
+            *reinterpret_cast<uint4*>(to + at) = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+        }
+        fence_proxy_async_smem();
+        warp_arrive(kw_ready, lane);
+        ok = true;
+      }
+    }
+  } else {
+    reg_inc<128>();
+    const int quarter = warp & 3, half = (warp - 12) >> 2;
+    const int r = quarter * 32 + lane;
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    const int col0 = half * kCols;
+    const bool holds = quarter * 32 < DK;
+    const bool row_ok = r < a.Dk && col0 < a.Dv;
+    uint32_t it = 0;
+    bool ok = true;
+    for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
+      const Unit u = decode_unit(args, unit);
+      float S[kCols];
+      const float* from = nullptr;
+      float* to = nullptr;
+      int64_t from_sc = 1, to_sc = 1;
+      if (row_ok) {
+        if (whole) {
+          if (a.first.data != nullptr) {
+            from_sc = a.first.stride_col;
+            from = a.first.data + u.b * a.first.stride_b + u.h * a.first.stride_h +
+                   r * a.first.stride_row + col0 * from_sc;
+          }
+          to_sc = a.last.stride_col;
+          to = a.last.data + u.b * a.last.stride_b + u.h * a.last.stride_h +
+               r * a.last.stride_row + col0 * to_sc;
+        } else {
+          to = args.split.states + (((u.seg * a.B + u.b) * a.H + u.h) * a.Dk + r) * a.Dv + col0;
+        }
+      }
+      load_memory_row<kCols>(from, from_sc, a.Dv - col0, S);
+      for (int i = 0; i < u.chunks; ++i, ++it) {
+        const int n = chunk_steps(u, chunk_t0(u, i, reverse));
+        ok = false;
+        if (!mbar_wait_bounded(delta_done, it & 1)) break;
+        tc_fence_after();
+        if (holds) {
+          const float gn = decay_pow(u.log2g, n);
+#pragma unroll
+          for (int c0 = 0; c0 < kCols; c0 += 16) {
+            uint32_t x[16];
+            tmem_ld16_issue(tmem + L::kDelta + lanes + col0 + c0, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              S[c0 + j] = fmaf(gn, S[c0 + j], a.kv_scale * __uint_as_float(x[j]));
+            }
+          }
+        }
+        tc_fence_before();
+        warp_arrive(delta_read, lane);
+        ok = true;
+      }
+      if (ok) store_memory_row<kCols>(to, to_sc, a.Dv - col0, S);
     }
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  if (warp == 1) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
-                 "r"(L::kTmemCols));
-  }
+  tmem_free(tmem, warp);
 }
 
 // A [d, t, h, b] map of 64 x 128 boxes; a dimension of stride 0 or size 1 has
@@ -654,32 +1029,42 @@ bool make_attn_map(CUtensorMap* map, const mb_steps& x, int64_t T, int64_t H, in
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DK, int DV, bool STATES_ONLY>
-int launch_chunks(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                  const TcArgs& args, cudaStream_t s) {
-  auto kern = attn_chunk_kernel<T, DK, DV, STATES_ONLY>;
-  constexpr size_t smem = TcLayout<DK, DV>::kSmem;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  const int64_t blocks = args.split.segments * args.a.B * args.a.H;
-  MB_CHECK_ARG(blocks <= 0x7fffffff, "mb_decay_attention: too many (batch, head) rows");
-  kern<<<static_cast<unsigned>(blocks), kTcThreads, smem, s>>>(mq, mk, mv, args);
-  MB_CHECK_LAUNCH("mb_decay_attention (chunks)");
-  return 0;
+int attn_sm_count() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) {
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  }
+  return n > 0 ? n : 148;
 }
 
 template <typename T, int DK, int DV>
-int launch_mode(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                const TcArgs& args, bool states_only, cudaStream_t s) {
-  return states_only ? launch_chunks<T, DK, DV, true>(mq, mk, mv, args, s)
-                     : launch_chunks<T, DK, DV, false>(mq, mk, mv, args, s);
+int launch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+              const TcArgs& args, bool states, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>(imin64(args.units, attn_sm_count()));
+  if (states) {
+    constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
+    constexpr size_t smem = StatesLayout<DK, DV, PARTS>::kSmem;
+    auto kern = attn_states_kernel<T, DK, DV>;
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    kern<<<grid, kTcThreads, smem, s>>>(mk, mv, args);
+    MB_CHECK_LAUNCH("mb_decay_attention (states)");
+  } else {
+    constexpr size_t smem = OutLayout<DK, DV>::kSmem;
+    auto kern = attn_out_kernel<T, DK, DV>;
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    kern<<<grid, kTcThreads, smem, s>>>(mq, mk, mv, args);
+    MB_CHECK_LAUNCH("mb_decay_attention (outputs)");
+  }
+  return 0;
 }
 
 template <typename T>
-int launch_type(const mb_decay_attention_args& a, const AttnSplit& split, bool states_only,
+int launch_type(const mb_decay_attention_args& a, const AttnSplit& split, bool states,
                 cudaStream_t s) {
   TcArgs args;
   args.a = a;
   args.split = split;
+  args.units = split.segments * a.B * a.H;
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   CUtensorMap mq, mk, mv;
   MB_CHECK_ARG(make_attn_map(&mq, a.q, a.T, a.H, a.B, a.Dk, bf16, &args.q_h, &args.q_b) &&
@@ -687,10 +1072,10 @@ int launch_type(const mb_decay_attention_args& a, const AttnSplit& split, bool s
                    make_attn_map(&mv, a.v, a.T, a.H, a.B, a.Dv, bf16, &args.v_h, &args.v_b),
                "mb_decay_attention: cuTensorMapEncodeTiled failed (shape or alignment)");
   const bool k64 = a.Dk <= 64, v64 = a.Dv <= 64;
-  if (k64 && v64) return launch_mode<T, 64, 64>(mq, mk, mv, args, states_only, s);
-  if (k64) return launch_mode<T, 64, 128>(mq, mk, mv, args, states_only, s);
-  if (v64) return launch_mode<T, 128, 64>(mq, mk, mv, args, states_only, s);
-  return launch_mode<T, 128, 128>(mq, mk, mv, args, states_only, s);
+  if (k64 && v64) return launch_tc<T, 64, 64>(mq, mk, mv, args, states, s);
+  if (k64) return launch_tc<T, 64, 128>(mq, mk, mv, args, states, s);
+  if (v64) return launch_tc<T, 128, 64>(mq, mk, mv, args, states, s);
+  return launch_tc<T, 128, 128>(mq, mk, mv, args, states, s);
 }
 
 // Rows that the tensor-map copies and 16-byte stores take: 16-byte base and strides.
@@ -733,10 +1118,10 @@ AttnSplit attn_tc_split(const mb_decay_attention_args& a) {
   return AttnSplit{static_cast<int>(best), best > 1 ? per * kC : a.T, nullptr};
 }
 
-int attn_tc_launch(const mb_decay_attention_args& a, const AttnSplit& split, bool states_only,
+int attn_tc_launch(const mb_decay_attention_args& a, const AttnSplit& split, bool states,
                    cudaStream_t stream) {
-  return a.dtype == MB_BF16 ? launch_type<__nv_bfloat16>(a, split, states_only, stream)
-                            : launch_type<__half>(a, split, states_only, stream);
+  return a.dtype == MB_BF16 ? launch_type<__nv_bfloat16>(a, split, states, stream)
+                            : launch_type<__half>(a, split, states, stream);
 }
 
 int attention_unit_status(bool clear) { return read_device_status(clear); }
