@@ -50,23 +50,29 @@ struct TcArgs {
   AttnSplit split;
   int64_t units;  // segments x B x H
   // whether a dimension's coordinate counts (0: the tensor is broadcast along it)
-  int32_t q_b, q_h, k_b, k_h, v_b, v_h;
+  int32_t q_b, q_h, k_b, k_h, v_b, v_h, o_b, o_h;
 };
 
 template <int DK, int DV>
 struct OutLayout {
+  // 128-wide heads fill shared memory: one V stage instead of two, and outputs are
+  // staged where their chunk's Q was
+  static constexpr bool kFull = DK == 128 && DV == 128;
+  static constexpr int kVStages = kFull ? 1 : 2;
   static constexpr int kQBytes = kC * DK * 2;
   static constexpr int kVBytes = kC * DV * 2;
-  static constexpr int kQ = 0;  // two stages each of Q, K and V
+  static constexpr int kQ = 0;  // two stages each of Q and K
   static constexpr int kK = kQ + 2 * kQBytes;
-  static constexpr int kV = kK + 2 * kQBytes;
-  static constexpr int kS = kV + 2 * kVBytes;
-  static constexpr int kWeights = kS + DK * DV * 2;      // weights of the scores by distance
-  static constexpr int kRowScale = kWeights + 256 * 4;   // fp16: 1 / scale of P's rows, by stage
+  static constexpr int kLo = kK + 2 * kQBytes;  // what rounding leaves of W_kv K
+  static constexpr int kV = kLo + kQBytes;
+  static constexpr int kS = kV + kVStages * kVBytes;
+  static constexpr int kO = kFull ? kQ : kS + DK * DV * 2;
+  static constexpr int kRowScale = kS + DK * DV * 2 + (kFull ? 0 : kVBytes);  // fp16: 1 / scale of
+                                                          // P's rows, by stage
   static constexpr int kRowTop = kRowScale + 2 * kC * 4;  // fp16: largest of the other half
   static constexpr int kMax = kRowTop + kC * 4;           // fp16: largest values of each warp
   static constexpr int kBars = kMax + 2 * 8 * 4;
-  static constexpr int kNumBars = 18;
+  static constexpr int kNumBars = 20;
   static constexpr size_t kSmem = kBars + kNumBars * 8 + 16;
   static_assert(kBars % 8 == 0 && kSmem <= 232448, "shared memory");
   // TMEM columns
@@ -95,7 +101,7 @@ struct Unit {
   int b, h;
   int64_t seg, lo, hi, end;
   int chunks;
-  float log2g;
+  float g, log2g;
 };
 
 __device__ __forceinline__ Unit decode_unit(const TcArgs& args, int64_t unit) {
@@ -108,7 +114,8 @@ __device__ __forceinline__ Unit decode_unit(const TcArgs& args, int64_t unit) {
   u.hi = imin64(a.T, u.lo + args.split.len);
   u.end = imin64(u.hi, attn_row_length(a.lengths, u.b, a.T));
   u.chunks = u.end > u.lo ? static_cast<int>((u.end - u.lo + kC - 1) / kC) : 0;
-  u.log2g = log2f(a.decay[u.h]);
+  u.g = a.decay[u.h];
+  u.log2g = log2f(u.g);
   return u;
 }
 
@@ -191,6 +198,16 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int d, int t,
+                                             int h, int b) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(d), "r"(t), "r"(h), "r"(b), "r"(smem_addr(src))
+      : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
@@ -227,8 +244,8 @@ __device__ __forceinline__ float fp16_scale(float top) {
   return __uint_as_float(static_cast<uint32_t>(s) << 23);
 }
 
-// Barriers 1..: 1 the score warps, 2 the carry warps, 3.. the two score warps of
-// one TMEM lane quarter.
+// Named barriers: 2 the carry warps, 3..6 the two score warps and 7..10 the two
+// output warps of one TMEM lane quarter.
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -311,6 +328,30 @@ __device__ __forceinline__ void store_memory_row(float* p, int64_t stride, int64
   }
 }
 
+// Sixteen scores of one row times c g^distance, zero on the other side of the
+// diagonal: column j of the group lies at distance e0 - j (REVERSE: j - e0) from the
+// row. The weight runs along the columns, one product each; MASKED: the group may
+// touch the diagonal (or, in reverse, column `valid`, where the row's steps end).
+// Selects, not products with zero: what lies outside may be infinite or NaN.
+template <bool REVERSE, bool MASKED>
+__device__ __forceinline__ void weigh16(const uint32_t (&v)[16], int e0, int valid, float c,
+                                        const Unit& u, float (&f)[16]) {
+  const int d = REVERSE ? -1 - e0 : e0 - 16;  // distance one step before the first column
+  float w = d >= 0 ? c * decay_pow(u.log2g, d) : 0.0f;
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    const int j = REVERSE ? x : 15 - x;
+    if constexpr (MASKED) {
+      w = j == e0 ? c : w * u.g;
+      const bool in = REVERSE ? j >= e0 && j < valid : j <= e0;
+      f[j] = in ? __uint_as_float(v[j]) * w : 0.0f;
+    } else {
+      w *= u.g;
+      f[j] = __uint_as_float(v[j]) * w;
+    }
+  }
+}
+
 // Values past the row's end may hold anything (0 * NaN must not reach a sum):
 // this thread's half of row r of a V tile becomes zero.
 template <int DV>
@@ -324,17 +365,17 @@ __device__ __forceinline__ void zero_v_row(uint8_t* vs, int r, int half) {
 // ---------------------------------------------------------------------------
 // Outputs
 // ---------------------------------------------------------------------------
-template <typename T, int DK, int DV>
+template <typename T, int DK, int DV, bool REVERSE>
 __global__ void __launch_bounds__(kTcThreads, 1)
     attn_out_kernel(const __grid_constant__ CUtensorMap map_q,
                     const __grid_constant__ CUtensorMap map_k,
                     const __grid_constant__ CUtensorMap map_v,
+                    const __grid_constant__ CUtensorMap map_o,
                     const __grid_constant__ TcArgs args) {
   using L = OutLayout<DK, DV>;
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr int kCols = DV / 2;  // memory and output columns per worker thread
   extern __shared__ __align__(1024) uint8_t smem[];
-  float* weights = reinterpret_cast<float*>(smem + L::kWeights);
   float* row_scale = reinterpret_cast<float*>(smem + L::kRowScale);
   float* row_top = reinterpret_cast<float*>(smem + L::kRowTop);
   float* warp_max = reinterpret_cast<float*>(smem + L::kMax);
@@ -342,21 +383,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* full_q = bars;            // [2]
   uint64_t* full_k = bars + 2;        // [2]
   uint64_t* full_v = bars + 4;        // [2]
-  uint64_t* empty = bars + 6;         // [2] a stage's Q, K and V
-  uint64_t* scores_done = bars + 8;
-  uint64_t* p_ready = bars + 9;
-  uint64_t* pv_done = bars + 10;
-  uint64_t* out_done = bars + 11;
-  uint64_t* out_read = bars + 12;
-  uint64_t* kw_ready = bars + 13;
-  uint64_t* delta_done = bars + 14;
-  uint64_t* carry_ready = bars + 15;
-  uint64_t* drained = bars + 16;
+  uint64_t* empty_q = bars + 6;       // [2] scores and Q S read it, outputs left it
+  uint64_t* empty_kv = bars + 8;      // [2] a chunk's K and V
+  uint64_t* scores_done = bars + 10;
+  uint64_t* p_ready = bars + 11;
+  uint64_t* pv_done = bars + 12;
+  uint64_t* out_done = bars + 13;
+  uint64_t* out_read = bars + 14;
+  uint64_t* kw_ready = bars + 15;
+  uint64_t* delta_done = bars + 16;
+  uint64_t* carry_ready = bars + 17;
+  uint64_t* drained = bars + 18;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
 
   const mb_decay_attention_args& a = args.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool reverse = a.reverse != 0;
+  constexpr bool reverse = REVERSE;
+  constexpr int VS = L::kVStages;
   // whether units start from a memory; without one their first chunk has no Q S
   const bool carry_in = args.split.segments > 1 || a.first.data != nullptr;
 
@@ -365,7 +408,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&full_q[s], 1);
       mbar_init(&full_k[s], 1);
       mbar_init(&full_v[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty_q[s], 8);
+      mbar_init(&empty_kv[s], 1);
     }
     mbar_init(scores_done, 1);
     mbar_init(p_ready, 8);
@@ -386,7 +430,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp < 4) {
     reg_dec<56>();
     if (warp == 0 && lane == 0) {
-      uint32_t it = 0;
+      uint32_t it = 0, nq = 0, nk = 0, nv = 0;  // loads issued
       bool ok = true;
       for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
         const Unit u = decode_unit(args, unit);
@@ -395,38 +439,50 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int i = 0; i < u.chunks; ++i, ++it) {
           const int s = it & 1;
           const int t = static_cast<int>(chunk_t0(u, i, reverse));
-          if (it >= 2 && !mbar_wait_bounded(&empty[s], ((it >> 1) - 1) & 1)) {
-            ok = false;
-            break;
-          }
+          ok = false;
+          if (it >= 2 && !mbar_wait_bounded(&empty_q[s], ((it >> 1) - 1) & 1)) break;
           mbar_arrive_expect_tx(&full_q[s], L::kQBytes);
-          mbar_arrive_expect_tx(&full_k[s], L::kQBytes);
-          mbar_arrive_expect_tx(&full_v[s], L::kVBytes);
 #pragma unroll
           for (int x = 0; x < DK / 64; ++x) {
             tma_load_4d(smem + L::kQ + s * L::kQBytes + x * kBlockBytes, &map_q, x * 64, t, qh, qb,
                         &full_q[s]);
+          }
+          nq = it + 1;
+          if (it >= 2 && !mbar_wait_bounded(&empty_kv[s], ((it >> 1) - 1) & 1)) break;
+          mbar_arrive_expect_tx(&full_k[s], L::kQBytes);
+#pragma unroll
+          for (int x = 0; x < DK / 64; ++x) {
             tma_load_4d(smem + L::kK + s * L::kQBytes + x * kBlockBytes, &map_k, x * 64, t, kh, kb,
                         &full_k[s]);
           }
+          nk = it + 1;
+          if (VS == 1 && it >= 1 && !mbar_wait_bounded(&empty_kv[s ^ 1], ((it - 1) >> 1) & 1)) break;
+          mbar_arrive_expect_tx(&full_v[it % VS], L::kVBytes);
 #pragma unroll
           for (int x = 0; x < DV / 64; ++x) {
-            tma_load_4d(smem + L::kV + s * L::kVBytes + x * kBlockBytes, &map_v, x * 64, t, vh, vb,
-                        &full_v[s]);
+            tma_load_4d(smem + L::kV + (it % VS) * L::kVBytes + x * kBlockBytes, &map_v, x * 64, t,
+                        vh, vb, &full_v[it % VS]);
           }
+          nv = it + 1;
+          ok = true;
         }
       }
       // every issued copy has landed before the CTA can retire
-      for (uint32_t j = it > 2 ? it - 2 : 0; j < it; ++j) {
+      for (uint32_t j = nq > 2 ? nq - 2 : 0; j < nq; ++j) {
         (void)mbar_wait_bounded(&full_q[j & 1], (j >> 1) & 1);
+      }
+      for (uint32_t j = nk > 2 ? nk - 2 : 0; j < nk; ++j) {
         (void)mbar_wait_bounded(&full_k[j & 1], (j >> 1) & 1);
-        (void)mbar_wait_bounded(&full_v[j & 1], (j >> 1) & 1);
+      }
+      for (uint32_t j = nv > VS ? nv - VS : 0; j < nv; ++j) {
+        (void)mbar_wait_bounded(&full_v[j % VS], (j / VS) & 1);
       }
     } else if (warp == 1 && lane == 0) {
       const uint32_t i_scores = tc_idesc<T>(kC, false, false);
       const uint32_t i_out = tc_idesc<T>(DV, false, true);
       const uint32_t i_delta = tc_idesc<T>(DV, true, true);
       const uint32_t sq = smem_addr(smem + L::kQ), sk = smem_addr(smem + L::kK);
+      const uint32_t slo = smem_addr(smem + L::kLo);
       const uint32_t sv = smem_addr(smem + L::kV), ss = smem_addr(smem + L::kS);
       uint32_t it = 0, hand = 0, cin = 0;
       bool ok = true;
@@ -460,13 +516,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int64_t following = next_unit(unit + gridDim.x);
         for (int i = 0; i < u.chunks; ++i, ++it) {
           const int s = it & 1;
-          const uint32_t v0 = sv + s * L::kVBytes;
+          const uint32_t v0 = sv + (it % VS) * L::kVBytes;
           const bool last = i + 1 == u.chunks;
           ok = false;
           // P is written, and the last chunk's outputs have been read
           if (!mbar_wait_bounded(p_ready, it & 1)) break;
           if (it >= 1 && !mbar_wait_bounded(out_read, (it - 1) & 1)) break;
-          if (!mbar_wait_bounded(&full_v[s], (it >> 1) & 1)) break;
+          if (!mbar_wait_bounded(&full_v[it % VS], (it / VS) & 1)) break;
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < kC / 16; ++k) {
@@ -499,12 +555,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const uint32_t k0 = sk + s * L::kQBytes;
 #pragma unroll
             for (int k = 0; k < kC / 16; ++k) {
-              mma_f16(tmem + L::kDelta, mn_desc(k0 + k * 2048, kBlockBytes),
+              mma_f16(tmem + L::kDelta, mn_desc(slo + k * 2048, kBlockBytes),
                       mn_desc(v0 + k * 2048, kBlockBytes), i_delta, k != 0);
+            }
+#pragma unroll
+            for (int k = 0; k < kC / 16; ++k) {
+              mma_f16(tmem + L::kDelta, mn_desc(k0 + k * 2048, kBlockBytes),
+                      mn_desc(v0 + k * 2048, kBlockBytes), i_delta, 1u);
             }
             mma_commit(delta_done);
           }
-          mma_commit(&empty[s]);
+          mma_commit(&empty_kv[s]);
           ok = true;
         }
         unit = following;
@@ -518,20 +579,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const int r = quarter * 32 + lane;
     const uint32_t t_scores = tmem + L::kScores + (uint32_t(quarter * 32) << 16);
-    const float* w_row = weights + 128 + r;  // w_row[-j]: weight of step j for this row
-    uint32_t it = 0;
+    const float intra = a.out_scale * a.kv_scale;
+    uint32_t it = 0, hand = 0;
     bool ok = true;
     for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
       const Unit u = decode_unit(args, unit);
-      if (u.chunks == 0) continue;
-      // weights[128 + r - j]: scale * g^|r - j| of the causal side, 0 of the other
-      bar_sync(1, kGroup);  // the last unit's have been read
-      {
-        const int x = threadIdx.x - 128;
-        const int d = reverse ? 128 - x : x - 128;
-        weights[x] = d >= 0 ? decay_pow(u.log2g, d) * (a.out_scale * a.kv_scale) : 0.0f;
-      }
-      bar_sync(1, kGroup);
       for (int i = 0; i < u.chunks; ++i, ++it) {
         const int s = it & 1;
         const int n = chunk_steps(u, chunk_t0(u, i, reverse));
@@ -539,16 +591,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         ok = false;
         if (!mbar_wait_bounded(&full_k[s], (it >> 1) & 1)) break;
         if (n < kC) {
-          if (!mbar_wait_bounded(&full_v[s], (it >> 1) & 1)) break;
-          if (r >= n) zero_v_row<DV>(smem + L::kV + s * L::kVBytes, r, half);
+          if (!mbar_wait_bounded(&full_v[it % VS], (it / VS) & 1)) break;
+          if (r >= n) zero_v_row<DV>(smem + L::kV + (it % VS) * L::kVBytes, r, half);
           fence_proxy_async_smem();
         }
         if (!mbar_wait_bounded(scores_done, it & 1)) break;
         tc_fence_after();
         // column blocks half and half + 2; those wholly on the other side of the
-        // diagonal are zero, and in reverse steps past the row's end are, too
+        // diagonal are zero
         auto blank = [&](int jb) { return reverse ? jb < quarter : jb > quarter; };
-        const int last = reverse ? n : kC;
+        auto group = [&](int jb, int y, float (&f)[16]) {  // columns jb * 32 + y ..
+          uint32_t v[16];
+          tmem_ld16_issue(t_scores + jb * 32 + y, v);
+          tmem_wait_ld();
+          const int e0 = r - jb * 32 - y;
+          if (jb == quarter || (reverse && n < kC)) {
+            weigh16<REVERSE, true>(v, e0, n - jb * 32 - y, intra, u, f);
+          } else {
+            weigh16<REVERSE, false>(v, e0, 16, intra, u, f);
+          }
+        };
         float scale = 1.0f;
         if constexpr (kHalf) {
           // fp16: P's rows are brought to a common magnitude by a power of two
@@ -557,17 +619,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int x = 0; x < 2; ++x) {
             const int jb = half + 2 * x;
             if (blank(jb)) continue;
-            const float* wj = w_row - jb * 32;
 #pragma unroll
             for (int y = 0; y < 32; y += 16) {
-              uint32_t v[16];
-              tmem_ld16_issue(t_scores + jb * 32 + y, v);
-              tmem_wait_ld();
+              float f[16];
+              group(jb, y, f);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float w = fabsf(__uint_as_float(v[j]) * wj[-(y + j)]);
-                top = fmaxf(top, jb * 32 + y + j < last ? w : 0.0f);  // drops a NaN
-              }
+              for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(f[j]));  // drops a NaN
             }
           }
           (half == 0 ? row_scale + s * kC : row_top)[r] = top;
@@ -582,27 +639,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int j = 0; j < 16; ++j) p[x][j] = 0;
           } else {
-            const float* wj = w_row - jb * 32;
 #pragma unroll
             for (int y = 0; y < 32; y += 16) {
-              uint32_t v[16];
-              tmem_ld16_issue(t_scores + jb * 32 + y, v);
-              float w[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                w[j] = jb * 32 + y + j < last ? wj[-(y + j)] : 0.0f;
-              }
-              tmem_wait_ld();
+              float f[16];
+              group(jb, y, f);
 #pragma unroll
               for (int j = 0; j < 16; j += 2) {
-                // selects: what a zero weight hides may be infinite or NaN
-                float f[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const float m = __uint_as_float(v[j + e]) * (kHalf ? w[j + e] * scale : w[j + e]);
-                  f[e] = w[j + e] != 0.0f ? m : 0.0f;
-                }
-                p[x][(y + j) / 2] = pack2<T>(f[0], f[1]);
+                p[x][(y + j) / 2] = kHalf ? pack2<T>(f[j] * scale, f[j + 1] * scale)
+                                          : pack2<T>(f[j], f[j + 1]);
               }
             }
           }
@@ -619,20 +663,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_before();
         warp_arrive(p_ready, lane);
         if (i + 1 < u.chunks) {
-          // K <- W_kv K for the carry; the scores that read K are complete
+          // K <- W_kv K for the carry (the scores that read K are complete), and
+          // what rounding leaves of it, once the last chunk's remainders are used
+          if (hand >= 1 && !mbar_wait_bounded(delta_done, (hand - 1) & 1)) break;
+          ++hand;
           const float w = r < n ? kv_weight(u, r, n, reverse) : 0.0f;
 #pragma unroll
           for (int q = 0; q < DK / 16; ++q) {
-            uint4* at = reinterpret_cast<uint4*>(ks + piece_at(r, half * (DK / 16) + q, kC));
-            const uint4 x = *at;
+            const int at = piece_at(r, half * (DK / 16) + q, kC);
+            const uint4 x = *reinterpret_cast<const uint4*>(ks + at);
             const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-            uint32_t y[4];
+            uint32_t y[4], z[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float2 f = unpack2<T>(in[e]);
-              y[e] = r < n ? pack2<T>(f.x * w, f.y * w) : 0u;
+              const float f0 = r < n ? f.x * w : 0.0f, f1 = r < n ? f.y * w : 0.0f;
+              y[e] = pack2<T>(f0, f1);
+              const float2 back = unpack2<T>(y[e]);
+              z[e] = pack2<T>(f0 - back.x, f1 - back.y);
             }
-            *at = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(ks + at) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(smem + L::kLo + at) = make_uint4(z[0], z[1], z[2], z[3]);
           }
           fence_proxy_async_smem();
           warp_arrive(kw_ready, lane);
@@ -711,15 +762,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int i = 0; i < u.chunks; ++i, ++it) {
         const int64_t t0 = chunk_t0(u, i, reverse);
         const int n = chunk_steps(u, t0);
+        const int s = it & 1;
         ok = false;
         if (!mbar_wait_bounded(out_done, it & 1)) break;
         tc_fence_after();
-        const float w_in = kHalf ? row_scale[(it & 1) * kC + r] : 1.0f;
+        const float w_in = kHalf ? row_scale[s * kC + r] : 1.0f;
         const bool inter = i > 0 || carry_in;
         const float w_out =
             r < n ? out_weight(u, r, n, reverse) * (a.out_scale * inv_s) : 0.0f;
-        const bool store = t0 + r < u.hi;  // steps past the row's length get zeros
-        T* row = o + (t0 + r) * a.o.stride_t + col0;
+        // staged as rows of 128 bytes: a block of 32 rows x 64 columns per warp, or
+        // per two warps of 32 columns each; the last store has left its block
+        uint8_t* block = smem + L::kO + (L::kFull ? s * L::kQBytes : 0) +
+                         (kCols == 64 ? (half * 4 + quarter) : quarter) * 4096;
+        if constexpr (!L::kFull) {
+          if (lane == 0) tma_store_wait_read<0>();
+          if (kCols == 64) __syncwarp();
+          else bar_sync(7 + quarter, 64);
+        }
 #pragma unroll
         for (int c0 = 0; c0 < kCols; c0 += 16) {
           uint32_t x[16], y[16];
@@ -742,15 +801,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             p[j] = r < n ? pack2<T>(v[0], v[1]) : 0u;
           }
-          if (store && col0 + c0 < a.Dv) {
-            *reinterpret_cast<uint4*>(row + c0) = make_uint4(p[0], p[1], p[2], p[3]);
-            if (col0 + c0 + 8 < a.Dv) {
-              *reinterpret_cast<uint4*>(row + c0 + 8) = make_uint4(p[4], p[5], p[6], p[7]);
-            }
+          // steps past the row's length are staged as zeros
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int q = (kCols == 64 ? 0 : half * 4) + c0 / 8 + e;
+            *reinterpret_cast<uint4*>(block + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+                make_uint4(p[4 * e], p[4 * e + 1], p[4 * e + 2], p[4 * e + 3]);
           }
         }
         tc_fence_before();
+        fence_proxy_async_smem();
         warp_arrive(out_read, lane);
+        if (kCols == 32) bar_sync(7 + quarter, 64);
+        if (lane == 0 && (kCols == 64 || half == 0)) {
+          const int c = kCols == 64 ? col0 : 0;
+          const int64_t t = t0 + quarter * 32;
+          if (t < u.hi && c < a.Dv) {
+            tma_store_4d(&map_o, block, c, static_cast<int>(t), u.h * args.o_h, u.b * args.o_b);
+          }
+        }
         if (i + 1 < u.chunks) {
           if (!mbar_wait_bounded(delta_done, hand & 1)) break;
           ++hand;
@@ -770,6 +839,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           put_carry();
         }
+        if (lane == 0) {  // Q's stage may be filled again
+          if (L::kFull) tma_store_wait_read<0>();
+          mbar_arrive(&empty_q[s]);
+        }
         ok = true;
       }
       // whole chunks past the row's length: zeros
@@ -780,6 +853,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
     }
+    if (lane == 0) tma_store_wait_all();
   }
   tmem_free(tmem, warp);
 }
@@ -1007,10 +1081,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tmem_free(tmem, warp);
 }
 
-// A [d, t, h, b] map of 64 x 128 boxes; a dimension of stride 0 or size 1 has
+// A [d, t, h, b] map of 64-column boxes of `rows` steps; a dimension of stride 0 or size 1 has
 // extent 1 and its coordinate multiplied by 0.
 bool make_attn_map(CUtensorMap* map, const mb_steps& x, int64_t T, int64_t H, int64_t B, int64_t D,
-                   bool bf16, int32_t* h_on, int32_t* b_on) {
+                   bool bf16, int rows, int32_t* h_on, int32_t* b_on) {
   auto fn = tma_encode_fn();
   if (fn == nullptr) return false;
   *h_on = H > 1 && x.stride_h != 0;
@@ -1021,7 +1095,7 @@ bool make_attn_map(CUtensorMap* map, const mb_steps& x, int64_t T, int64_t H, in
   cuuint64_t strides[3] = {static_cast<cuuint64_t>(T > 1 ? x.stride_t * 2 : 16),
                            static_cast<cuuint64_t>(*h_on ? x.stride_h * 2 : 16),
                            static_cast<cuuint64_t>(*b_on ? x.stride_b * 2 : 16)};
-  cuuint32_t box[4] = {64, kC, 1, 1};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1};
   cuuint32_t estride[4] = {1, 1, 1, 1};
   return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
             x.data, dims, strides, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -1039,7 +1113,7 @@ int attn_sm_count() {
 
 template <typename T, int DK, int DV>
 int launch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-              const TcArgs& args, bool states, cudaStream_t s) {
+              const CUtensorMap& mo, const TcArgs& args, bool states, cudaStream_t s) {
   const unsigned grid = static_cast<unsigned>(imin64(args.units, attn_sm_count()));
   if (states) {
     constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
@@ -1050,9 +1124,10 @@ int launch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& m
     MB_CHECK_LAUNCH("mb_decay_attention (states)");
   } else {
     constexpr size_t smem = OutLayout<DK, DV>::kSmem;
-    auto kern = attn_out_kernel<T, DK, DV>;
+    auto kern = args.a.reverse != 0 ? attn_out_kernel<T, DK, DV, true>
+                                    : attn_out_kernel<T, DK, DV, false>;
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    kern<<<grid, kTcThreads, smem, s>>>(mq, mk, mv, args);
+    kern<<<grid, kTcThreads, smem, s>>>(mq, mk, mv, mo, args);
     MB_CHECK_LAUNCH("mb_decay_attention (outputs)");
   }
   return 0;
@@ -1066,33 +1141,35 @@ int launch_type(const mb_decay_attention_args& a, const AttnSplit& split, bool s
   args.split = split;
   args.units = split.segments * a.B * a.H;
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-  CUtensorMap mq, mk, mv;
-  MB_CHECK_ARG(make_attn_map(&mq, a.q, a.T, a.H, a.B, a.Dk, bf16, &args.q_h, &args.q_b) &&
-                   make_attn_map(&mk, a.k, a.T, a.H, a.B, a.Dk, bf16, &args.k_h, &args.k_b) &&
-                   make_attn_map(&mv, a.v, a.T, a.H, a.B, a.Dv, bf16, &args.v_h, &args.v_b),
+  CUtensorMap mq, mk, mv, mo;
+  MB_CHECK_ARG(make_attn_map(&mq, a.q, a.T, a.H, a.B, a.Dk, bf16, kC, &args.q_h, &args.q_b) &&
+                   make_attn_map(&mk, a.k, a.T, a.H, a.B, a.Dk, bf16, kC, &args.k_h, &args.k_b) &&
+                   make_attn_map(&mv, a.v, a.T, a.H, a.B, a.Dv, bf16, kC, &args.v_h, &args.v_b) &&
+                   make_attn_map(&mo, a.o, a.T, a.H, a.B, a.Dv, bf16, 32, &args.o_h, &args.o_b),
                "mb_decay_attention: cuTensorMapEncodeTiled failed (shape or alignment)");
   const bool k64 = a.Dk <= 64, v64 = a.Dv <= 64;
-  if (k64 && v64) return launch_tc<T, 64, 64>(mq, mk, mv, args, states, s);
-  if (k64) return launch_tc<T, 64, 128>(mq, mk, mv, args, states, s);
-  if (v64) return launch_tc<T, 128, 64>(mq, mk, mv, args, states, s);
-  return launch_tc<T, 128, 128>(mq, mk, mv, args, states, s);
+  if (k64 && v64) return launch_tc<T, 64, 64>(mq, mk, mv, mo, args, states, s);
+  if (k64) return launch_tc<T, 64, 128>(mq, mk, mv, mo, args, states, s);
+  if (v64) return launch_tc<T, 128, 64>(mq, mk, mv, mo, args, states, s);
+  return launch_tc<T, 128, 128>(mq, mk, mv, mo, args, states, s);
 }
 
 // Rows that the tensor-map copies and 16-byte stores take: 16-byte base and strides.
-bool steps_ok(const mb_steps& x, int64_t T, bool broadcast_ok) {
+bool steps_ok(const mb_steps& x, int64_t T) {
   const int64_t limit = int64_t(1) << 38;  // strides below 2^40 bytes
   return aligned_to(x.data, 16) && x.stride_t % 8 == 0 && x.stride_h % 8 == 0 &&
          x.stride_b % 8 == 0 && x.stride_t >= 0 && x.stride_h >= 0 && x.stride_b >= 0 &&
          x.stride_t < limit && x.stride_h < limit && x.stride_b < limit &&
-         (T <= 1 || x.stride_t > 0) && broadcast_ok;
+         (T <= 1 || x.stride_t > 0);
 }
 
 }  // namespace
 
 bool attn_tc_supported(const mb_decay_attention_args& a) {
   if (a.dtype == MB_F32 || a.Dk > 128 || a.Dv > 128 || a.T < kTcMinSteps) return false;
-  return a.Dv % 8 == 0 && steps_ok(a.q, a.T, true) && steps_ok(a.k, a.T, true) &&
-         steps_ok(a.v, a.T, true) && steps_ok(a.o, a.T, true);
+  const bool o_dense = (a.H == 1 || a.o.stride_h > 0) && (a.B == 1 || a.o.stride_b > 0);
+  return a.Dv % 8 == 0 && o_dense && steps_ok(a.q, a.T) && steps_ok(a.k, a.T) &&
+         steps_ok(a.v, a.T) && steps_ok(a.o, a.T);
 }
 
 // Segments of the time axis, in whole chunks: the count whose waves of CTAs (one
