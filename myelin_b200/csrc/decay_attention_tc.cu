@@ -12,10 +12,10 @@
 //
 // All products are tcgen05 (M = 128 steps or memory rows, sums in TMEM). 20 warps:
 //   warp 0      copies: Q, K, V, two stages of 128-byte-swizzled tiles
-//   warp 1      issues the products, one thread: P V, Q S, the next chunk's Q K^T,
-//               then (W_kv K)^T V
-//   warps 4-11  scores -> P (16 bits, back into TMEM as an A operand) and K -> W_kv K
-//               in place; two warps per 32 rows, half of the columns each
+//   warp 1      issues the products, one thread: Q S, (W_kv K)^T V, P V, then the next
+//               chunk's Q K^T
+//   warps 4-11  K -> W_kv K in place, then scores -> P (16 bits, back into TMEM as an
+//               A operand); two warps per 32 rows, half of the columns each
 //   warps 12-19 outputs; the carry in fp32 registers (row per lane, half of the
 //               columns), rounded into shared memory as the next chunk's operand
 // Registers move from the first three warpgroups to the last two (setmaxnreg).
@@ -90,7 +90,7 @@ struct StatesLayout {
   static constexpr int kLo = kK + 2 * kKBytes;  // the further parts of W_kv K
   static constexpr int kV = kLo + (PARTS - 1) * kKBytes;
   static constexpr int kBars = kV + 2 * kVBytes;
-  static constexpr int kNumBars = 10;
+  static constexpr int kNumBars = 12;
   static constexpr size_t kSmem = kBars + kNumBars * 8 + 16;
   static_assert(kSmem <= 232448, "shared memory");
   static constexpr uint32_t kDelta = 0;
@@ -228,6 +228,33 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   }
 }
 
+// Two fp32 products or sums in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
+        "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
+// One lane of a converged warp, the same each time; the compiler knows that the
+// code under it runs in one thread (products issue from uniform registers).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 // Byte offset of 16-byte piece `q` (8 columns) of row r in a 128-byte-swizzled
 // tile of `rows` rows whose 64-column blocks follow one another.
 __device__ __forceinline__ int piece_at(int r, int q, int rows) {
@@ -256,6 +283,34 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   if (lane == 0) mbar_arrive(bar);
 }
 
+
+// This thread's half of row r of a K tile times w (zero past the chunk's n steps), as
+// PARTS 16-bit parts that add up to it: the first in place, the others to `lo`.
+template <typename T, int DK, int PARTS>
+__device__ __forceinline__ void weigh_k_row(uint8_t* ks, uint8_t* lo, int r, int half, float w,
+                                            bool valid) {
+  const float2 w2 = make_float2(w, w), minus = make_float2(-1.0f, -1.0f);
+#pragma unroll
+  for (int q = 0; q < DK / 16; ++q) {
+    const int at = piece_at(r, half * (DK / 16) + q, kC);
+    const uint4 x = *reinterpret_cast<const uint4*>(ks + at);
+    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+    float2 f[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = mul2(unpack2<T>(valid ? in[e] : 0u), w2);
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+      uint32_t y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        y[e] = pack2<T>(f[e].x, f[e].y);
+        if (part + 1 < PARTS) f[e] = fma2(unpack2<T>(y[e]), minus, f[e]);
+      }
+      uint8_t* to = part == 0 ? ks : lo + (part - 1) * kC * DK * 2;
+      *reinterpret_cast<uint4*>(to + at) = make_uint4(y[0], y[1], y[2], y[3]);
+    }
+  }
+}
 
 template <int N>
 __device__ __forceinline__ void reg_dec() {
@@ -334,7 +389,7 @@ __device__ __forceinline__ void store_memory_row(float* p, int64_t stride, int64
 // touch the diagonal (or, in reverse, column `valid`, where the row's steps end).
 // Selects, not products with zero: what lies outside may be infinite or NaN.
 template <bool REVERSE, bool MASKED>
-__device__ __forceinline__ void weigh16(const uint32_t (&v)[16], int e0, int valid, float c,
+__device__ __forceinline__ void weigh16(const uint32_t* v, int e0, int valid, float c,
                                         const Unit& u, float (&f)[16]) {
   const int d = REVERSE ? -1 - e0 : e0 - 16;  // distance one step before the first column
   float w = d >= 0 ? c * decay_pow(u.log2g, d) : 0.0f;
@@ -387,17 +442,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* empty_kv = bars + 8;      // [2] a chunk's K and V
   uint64_t* scores_done = bars + 10;
   uint64_t* p_ready = bars + 11;
-  uint64_t* pv_done = bars + 12;
-  uint64_t* out_done = bars + 13;
-  uint64_t* out_read = bars + 14;
-  uint64_t* kw_ready = bars + 15;
-  uint64_t* delta_done = bars + 16;
-  uint64_t* carry_ready = bars + 17;
-  uint64_t* drained = bars + 18;
+  uint64_t* out_done = bars + 12;
+  uint64_t* out_read = bars + 13;
+  uint64_t* kw_ready = bars + 14;
+  uint64_t* delta_done = bars + 15;
+  uint64_t* carry_ready = bars + 16;
+  uint64_t* drained = bars + 17;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
 
   const mb_decay_attention_args& a = args.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr bool reverse = REVERSE;
   constexpr int VS = L::kVStages;
   // whether units start from a memory; without one their first chunk has no Q S
@@ -413,7 +467,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     mbar_init(scores_done, 1);
     mbar_init(p_ready, 8);
-    mbar_init(pv_done, 1);
     mbar_init(out_done, 2);  // the products' completion, and what their operands' makers wrote
     mbar_init(out_read, 8);
     mbar_init(kw_ready, 8);
@@ -429,7 +482,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // that a carry enters. All roles count alike.
   if (warp < 4) {
     reg_dec<56>();
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
       uint32_t it = 0, nq = 0, nk = 0, nv = 0;  // loads issued
       bool ok = true;
       for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
@@ -440,14 +493,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int s = it & 1;
           const int t = static_cast<int>(chunk_t0(u, i, reverse));
           ok = false;
-          if (it >= 2 && !mbar_wait_bounded(&empty_q[s], ((it >> 1) - 1) & 1)) break;
-          mbar_arrive_expect_tx(&full_q[s], L::kQBytes);
-#pragma unroll
-          for (int x = 0; x < DK / 64; ++x) {
-            tma_load_4d(smem + L::kQ + s * L::kQBytes + x * kBlockBytes, &map_q, x * 64, t, qh, qb,
-                        &full_q[s]);
-          }
-          nq = it + 1;
           if (it >= 2 && !mbar_wait_bounded(&empty_kv[s], ((it >> 1) - 1) & 1)) break;
           mbar_arrive_expect_tx(&full_k[s], L::kQBytes);
 #pragma unroll
@@ -456,6 +501,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         &full_k[s]);
           }
           nk = it + 1;
+          if (it >= 2 && !mbar_wait_bounded(&empty_q[s], ((it >> 1) - 1) & 1)) break;
+          mbar_arrive_expect_tx(&full_q[s], L::kQBytes);
+#pragma unroll
+          for (int x = 0; x < DK / 64; ++x) {
+            tma_load_4d(smem + L::kQ + s * L::kQBytes + x * kBlockBytes, &map_q, x * 64, t, qh, qb,
+                        &full_q[s]);
+          }
+          nq = it + 1;
           if (VS == 1 && it >= 1 && !mbar_wait_bounded(&empty_kv[s ^ 1], ((it - 1) >> 1) & 1)) break;
           mbar_arrive_expect_tx(&full_v[it % VS], L::kVBytes);
 #pragma unroll
@@ -477,13 +530,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (uint32_t j = nv > VS ? nv - VS : 0; j < nv; ++j) {
         (void)mbar_wait_bounded(&full_v[j % VS], (j / VS) & 1);
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1 && elect_one()) {
       const uint32_t i_scores = tc_idesc<T>(kC, false, false);
       const uint32_t i_out = tc_idesc<T>(DV, false, true);
       const uint32_t i_delta = tc_idesc<T>(DV, true, true);
-      const uint32_t sq = smem_addr(smem + L::kQ), sk = smem_addr(smem + L::kK);
-      const uint32_t slo = smem_addr(smem + L::kLo);
-      const uint32_t sv = smem_addr(smem + L::kV), ss = smem_addr(smem + L::kS);
+      // descriptors of the tiles' starts: a step along a tile adds its bytes / 16
+      const uint64_t dq = sw128_kmajor_desc(smem_addr(smem + L::kQ));
+      const uint64_t dk = sw128_kmajor_desc(smem_addr(smem + L::kK));
+      const uint64_t dkt = mn_desc(smem_addr(smem + L::kK), kBlockBytes);
+      const uint64_t dlo = mn_desc(smem_addr(smem + L::kLo), kBlockBytes);
+      const uint64_t dv = mn_desc(smem_addr(smem + L::kV), kBlockBytes);
+      const uint64_t ds = mn_desc(smem_addr(smem + L::kS), DK * 128);
       uint32_t it = 0, hand = 0, cin = 0;
       bool ok = true;
       auto scores = [&](uint32_t j) {
@@ -495,9 +552,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < DK / 16; ++k) {
-          const uint32_t at = s * L::kQBytes + (k >> 2) * kBlockBytes + (k & 3) * 32;
-          mma_f16(tmem + L::kScores, sw128_kmajor_desc(sq + at), sw128_kmajor_desc(sk + at),
-                  i_scores, k != 0);
+          const uint32_t at = (s * L::kQBytes + (k >> 2) * kBlockBytes + (k & 3) * 32) >> 4;
+          mma_f16(tmem + L::kScores, dq + at, dk + at, i_scores, k != 0);
         }
         mma_commit(scores_done);
         return true;
@@ -516,56 +572,52 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int64_t following = next_unit(unit + gridDim.x);
         for (int i = 0; i < u.chunks; ++i, ++it) {
           const int s = it & 1;
-          const uint32_t v0 = sv + (it % VS) * L::kVBytes;
+          const uint64_t v0 = dv + (((it % VS) * L::kVBytes) >> 4);
           const bool last = i + 1 == u.chunks;
           ok = false;
-          // P is written, and the last chunk's outputs have been read
-          if (!mbar_wait_bounded(p_ready, it & 1)) break;
+          // what the output accumulators held has been read
           if (it >= 1 && !mbar_wait_bounded(out_read, (it - 1) & 1)) break;
-          if (!mbar_wait_bounded(&full_v[it % VS], (it / VS) & 1)) break;
-          tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < kC / 16; ++k) {
-            mma_f16_ts(tmem + L::kIntra, tmem + L::kScores + k * 8,
-                       mn_desc(v0 + k * 2048, kBlockBytes), i_out, k != 0);
-          }
-          mma_commit(pv_done);
           if (i > 0 || carry_in) {
             if (!mbar_wait_bounded(carry_ready, cin & 1)) break;
             ++cin;
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < DK / 16; ++k) {
-              mma_f16(tmem + L::kInter,
-                      sw128_kmajor_desc(sq + s * L::kQBytes + (k >> 2) * kBlockBytes + (k & 3) * 32),
-                      mn_desc(ss + k * 2048, DK * 128), i_out, k != 0);
+              const uint32_t at = (s * L::kQBytes + (k >> 2) * kBlockBytes + (k & 3) * 32) >> 4;
+              mma_f16(tmem + L::kInter, dq + at, ds + k * 128, i_out, k != 0);
             }
-          }
-          mma_commit(out_done);
-          mbar_arrive(out_done);
-          if (!last || following < args.units) {
-            // the next scores overwrite P: its product has to be complete
-            if (!mbar_wait_bounded(pv_done, it & 1)) break;
-            if (!scores(it + 1)) break;
           }
           if (!last) {
             if (!mbar_wait_bounded(kw_ready, hand & 1)) break;
             ++hand;
+            if (!mbar_wait_bounded(&full_v[it % VS], (it / VS) & 1)) break;
             tc_fence_after();
-            const uint32_t k0 = sk + s * L::kQBytes;
+            const uint64_t k0 = dkt + ((s * L::kQBytes) >> 4);
 #pragma unroll
             for (int k = 0; k < kC / 16; ++k) {
-              mma_f16(tmem + L::kDelta, mn_desc(slo + k * 2048, kBlockBytes),
-                      mn_desc(v0 + k * 2048, kBlockBytes), i_delta, k != 0);
+              mma_f16(tmem + L::kDelta, dlo + k * 128, v0 + k * 128, i_delta, k != 0);
             }
 #pragma unroll
             for (int k = 0; k < kC / 16; ++k) {
-              mma_f16(tmem + L::kDelta, mn_desc(k0 + k * 2048, kBlockBytes),
-                      mn_desc(v0 + k * 2048, kBlockBytes), i_delta, 1u);
+              mma_f16(tmem + L::kDelta, k0 + k * 128, v0 + k * 128, i_delta, 1u);
             }
             mma_commit(delta_done);
           }
+          if (!mbar_wait_bounded(p_ready, it & 1)) break;
+          if (!mbar_wait_bounded(&full_v[it % VS], (it / VS) & 1)) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < kC / 16; ++k) {
+            mma_f16_ts(tmem + L::kIntra, tmem + L::kScores + k * 8, v0 + k * 128, i_out, k != 0);
+          }
+          mma_commit(out_done);
           mma_commit(&empty_kv[s]);
+          mbar_arrive(out_done);
+          if (!last || following < args.units) {
+            // the next scores overwrite P: its product has to be complete
+            if (!mbar_wait_bounded(out_done, it & 1)) break;
+            if (!scores(it + 1)) break;
+          }
           ok = true;
         }
         unit = following;
@@ -580,16 +632,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int r = quarter * 32 + lane;
     const uint32_t t_scores = tmem + L::kScores + (uint32_t(quarter * 32) << 16);
     const float intra = a.out_scale * a.kv_scale;
-    uint32_t it = 0, hand = 0;
+    uint32_t it = 0;
     bool ok = true;
     for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
       const Unit u = decode_unit(args, unit);
       for (int i = 0; i < u.chunks; ++i, ++it) {
         const int s = it & 1;
         const int n = chunk_steps(u, chunk_t0(u, i, reverse));
-        uint8_t* ks = smem + L::kK + s * L::kQBytes;
         ok = false;
-        if (!mbar_wait_bounded(&full_k[s], (it >> 1) & 1)) break;
         if (n < kC) {
           if (!mbar_wait_bounded(&full_v[it % VS], (it / VS) & 1)) break;
           if (r >= n) zero_v_row<DV>(smem + L::kV + (it % VS) * L::kVBytes, r, half);
@@ -600,15 +650,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // column blocks half and half + 2; those wholly on the other side of the
         // diagonal are zero
         auto blank = [&](int jb) { return reverse ? jb < quarter : jb > quarter; };
-        auto group = [&](int jb, int y, float (&f)[16]) {  // columns jb * 32 + y ..
-          uint32_t v[16];
-          tmem_ld16_issue(t_scores + jb * 32 + y, v);
-          tmem_wait_ld();
+        auto group = [&](const uint32_t* v, int jb, int y, float (&f)[16]) {  // columns jb * 32 + y ..
           const int e0 = r - jb * 32 - y;
           if (jb == quarter || (reverse && n < kC)) {
-            weigh16<REVERSE, true>(v, e0, n - jb * 32 - y, intra, u, f);
+            weigh16<REVERSE, true>(v + y, e0, n - jb * 32 - y, intra, u, f);
           } else {
-            weigh16<REVERSE, false>(v, e0, 16, intra, u, f);
+            weigh16<REVERSE, false>(v + y, e0, 16, intra, u, f);
           }
         };
         float scale = 1.0f;
@@ -619,10 +666,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int x = 0; x < 2; ++x) {
             const int jb = half + 2 * x;
             if (blank(jb)) continue;
+            uint32_t v[32];
+            tmem_ld32_issue(t_scores + jb * 32, v);
+            tmem_wait_ld();
 #pragma unroll
             for (int y = 0; y < 32; y += 16) {
               float f[16];
-              group(jb, y, f);
+              group(v, jb, y, f);
 #pragma unroll
               for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(f[j]));  // drops a NaN
             }
@@ -639,10 +689,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int j = 0; j < 16; ++j) p[x][j] = 0;
           } else {
+            uint32_t v[32];
+            tmem_ld32_issue(t_scores + jb * 32, v);
+            tmem_wait_ld();
 #pragma unroll
             for (int y = 0; y < 32; y += 16) {
               float f[16];
-              group(jb, y, f);
+              group(v, jb, y, f);
 #pragma unroll
               for (int j = 0; j < 16; j += 2) {
                 p[x][(y + j) / 2] = kHalf ? pack2<T>(f[j] * scale, f[j + 1] * scale)
@@ -662,32 +715,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_wait_st();
         tc_fence_before();
         warp_arrive(p_ready, lane);
-        if (i + 1 < u.chunks) {
-          // K <- W_kv K for the carry (the scores that read K are complete), and
-          // what rounding leaves of it, once the last chunk's remainders are used
-          if (hand >= 1 && !mbar_wait_bounded(delta_done, (hand - 1) & 1)) break;
-          ++hand;
-          const float w = r < n ? kv_weight(u, r, n, reverse) : 0.0f;
-#pragma unroll
-          for (int q = 0; q < DK / 16; ++q) {
-            const int at = piece_at(r, half * (DK / 16) + q, kC);
-            const uint4 x = *reinterpret_cast<const uint4*>(ks + at);
-            const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-            uint32_t y[4], z[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 f = unpack2<T>(in[e]);
-              const float f0 = r < n ? f.x * w : 0.0f, f1 = r < n ? f.y * w : 0.0f;
-              y[e] = pack2<T>(f0, f1);
-              const float2 back = unpack2<T>(y[e]);
-              z[e] = pack2<T>(f0 - back.x, f1 - back.y);
-            }
-            *reinterpret_cast<uint4*>(ks + at) = make_uint4(y[0], y[1], y[2], y[3]);
-            *reinterpret_cast<uint4*>(smem + L::kLo + at) = make_uint4(z[0], z[1], z[2], z[3]);
-          }
-          fence_proxy_async_smem();
-          warp_arrive(kw_ready, lane);
-        }
         ok = true;
       }
     }
@@ -759,17 +786,59 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // the last unit's operand has been read: its outputs were complete
         if (carry_in) put_carry();
       }
+      bool owed = false;
       for (int i = 0; i < u.chunks; ++i, ++it) {
         const int64_t t0 = chunk_t0(u, i, reverse);
         const int n = chunk_steps(u, t0);
         const int s = it & 1;
         ok = false;
+        const float inv_now = inv_s;  // of the operand behind this chunk's Q S
+        auto release = [&]() {  // the last chunk's Q stage: its outputs have left it
+          if (L::kFull && owed && lane == 0) {
+            tma_store_wait_read<0>();
+            mbar_arrive(&empty_q[s ^ 1]);
+          }
+          owed = false;
+        };
+        if (i + 1 < u.chunks) {
+          // K <- W_kv K once the scores that read K are complete, and what rounding
+          // leaves of it (the last chunk's remainders are used: its D was waited for)
+          if (!mbar_wait_bounded(&full_k[s], (it >> 1) & 1)) break;
+          if (!mbar_wait_bounded(scores_done, it & 1)) break;
+          if (n < kC) {  // V as the score warps leave it
+            if (!mbar_wait_bounded(&full_v[it % VS], (it / VS) & 1)) break;
+            if (r >= n) zero_v_row<DV>(smem + L::kV + (it % VS) * L::kVBytes, r, half);
+          }
+          weigh_k_row<T, DK, 2>(smem + L::kK + s * L::kQBytes, smem + L::kLo, r, half,
+                                r < n ? kv_weight(u, r, n, reverse) : 0.0f, r < n);
+          fence_proxy_async_smem();
+          warp_arrive(kw_ready, lane);
+          release();
+          if (!mbar_wait_bounded(delta_done, hand & 1)) break;
+          ++hand;
+          tc_fence_after();
+          if (holds) {
+            const float gn = decay_pow(u.log2g, n);
+#pragma unroll
+            for (int c0 = 0; c0 < kCols; c0 += 16) {
+              uint32_t x[16];
+              tmem_ld16_issue(tmem + L::kDelta + lanes + col0 + c0, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                S[c0 + j] = fmaf(gn, S[c0 + j], a.kv_scale * __uint_as_float(x[j]));
+              }
+            }
+          }
+          put_carry();
+        }
+        release();
         if (!mbar_wait_bounded(out_done, it & 1)) break;
         tc_fence_after();
         const float w_in = kHalf ? row_scale[s * kC + r] : 1.0f;
         const bool inter = i > 0 || carry_in;
         const float w_out =
-            r < n ? out_weight(u, r, n, reverse) * (a.out_scale * inv_s) : 0.0f;
+            r < n ? out_weight(u, r, n, reverse) * (a.out_scale * inv_now) : 0.0f;
         // staged as rows of 128 bytes: a block of 32 rows x 64 columns per warp, or
         // per two warps of 32 columns each; the last store has left its block
         uint8_t* block = smem + L::kO + (L::kFull ? s * L::kQBytes : 0) +
@@ -820,26 +889,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tma_store_4d(&map_o, block, c, static_cast<int>(t), u.h * args.o_h, u.b * args.o_b);
           }
         }
-        if (i + 1 < u.chunks) {
-          if (!mbar_wait_bounded(delta_done, hand & 1)) break;
-          ++hand;
-          tc_fence_after();
-          if (holds) {
-            const float gn = decay_pow(u.log2g, n);
-#pragma unroll
-            for (int c0 = 0; c0 < kCols; c0 += 16) {
-              uint32_t x[16];
-              tmem_ld16_issue(tmem + L::kDelta + lanes + col0 + c0, x);
-              tmem_wait_ld();
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                S[c0 + j] = fmaf(gn, S[c0 + j], a.kv_scale * __uint_as_float(x[j]));
-              }
-            }
-          }
-          put_carry();
-        }
-        if (lane == 0) {  // Q's stage may be filled again
+        if (L::kFull && i + 1 < u.chunks) {
+          owed = true;  // Q's stage is released under the next chunk's work
+        } else if (lane == 0) {
           if (L::kFull) tma_store_wait_read<0>();
           mbar_arrive(&empty_q[s]);
         }
@@ -875,14 +927,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* full_k = bars;      // [2]
   uint64_t* full_v = bars + 2;  // [2]
   uint64_t* empty = bars + 4;   // [2]
-  uint64_t* kw_ready = bars + 6;
-  uint64_t* delta_done = bars + 7;
-  uint64_t* delta_read = bars + 8;
-  uint64_t* drained = bars + 9;
+  uint64_t* kw_ready = bars + 6;   // [2] steps 0..63 and 64..127 of a chunk
+  uint64_t* kw_used = bars + 8;    // [2] their products are complete
+  uint64_t* delta_read = bars + 10;
+  uint64_t* drained = bars + 11;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
 
   const mb_decay_attention_args& a = args.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const bool reverse = a.reverse != 0;
   const bool whole = args.split.segments == 1;
 
@@ -891,9 +943,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&full_k[s], 1);
       mbar_init(&full_v[s], 1);
       mbar_init(&empty[s], 1);
+      mbar_init(&kw_ready[s], 4);
+      mbar_init(&kw_used[s], 1);
     }
-    mbar_init(kw_ready, 8);
-    mbar_init(delta_done, 1);
     mbar_init(delta_read, 8);
     mbar_init(drained, 1);
     fence_barrier_init();
@@ -902,7 +954,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (warp < 4) {
     reg_dec<56>();
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
       uint32_t it = 0;
       bool ok = true;
       for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
@@ -934,10 +986,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         (void)mbar_wait_bounded(&full_k[j & 1], (j >> 1) & 1);
         (void)mbar_wait_bounded(&full_v[j & 1], (j >> 1) & 1);
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1 && elect_one()) {
       const uint32_t i_delta = tc_idesc<T>(DV, true, true);
-      const uint32_t sk = smem_addr(smem + L::kK), slo = smem_addr(smem + L::kLo);
-      const uint32_t sv = smem_addr(smem + L::kV);
+      const uint64_t dk = mn_desc(smem_addr(smem + L::kK), kBlockBytes);
+      const uint64_t dlo = mn_desc(smem_addr(smem + L::kLo), kBlockBytes);
+      const uint64_t dv = mn_desc(smem_addr(smem + L::kV), kBlockBytes);
       uint32_t it = 0;
       bool ok = true;
       for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
@@ -945,26 +998,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int i = 0; i < u.chunks; ++i, ++it) {
           const int s = it & 1;
           ok = false;
-          if (!mbar_wait_bounded(kw_ready, it & 1)) break;
           if (!mbar_wait_bounded(&full_v[s], (it >> 1) & 1)) break;
           if (it >= 1 && !mbar_wait_bounded(delta_read, (it - 1) & 1)) break;
-          tc_fence_after();
-          const uint32_t v0 = sv + s * L::kVBytes;
-          // the smallest parts first
+          const uint64_t k0 = dk + ((s * L::kKBytes) >> 4), v0 = dv + ((s * L::kVBytes) >> 4);
 #pragma unroll
-          for (int part = PARTS - 1; part >= 0; --part) {
-            const uint32_t k0 =
-                part == 0 ? sk + s * L::kKBytes : slo + (part - 1) * L::kKBytes;
+          for (int x = 0; x < 2; ++x) {
+            if (!mbar_wait_bounded(&kw_ready[x], it & 1)) break;
+            tc_fence_after();
 #pragma unroll
-            for (int k = 0; k < kC / 16; ++k) {
-              mma_f16(tmem + L::kDelta, mn_desc(k0 + k * 2048, kBlockBytes),
-                      mn_desc(v0 + k * 2048, kBlockBytes), i_delta,
-                      (part != PARTS - 1 || k != 0) ? 1u : 0u);
+            for (int part = PARTS - 1; part >= 0; --part) {  // the smallest parts first
+              const uint64_t p0 = part == 0 ? k0 : dlo + (((part - 1) * L::kKBytes) >> 4);
+#pragma unroll
+              for (int k = 4 * x; k < 4 * x + 4; ++k) {
+                mma_f16(tmem + L::kDelta, p0 + k * 128, v0 + k * 128, i_delta,
+                        (x != 0 || part != PARTS - 1 || k != 0) ? 1u : 0u);
+              }
             }
+            mma_commit(&kw_used[x]);
+            ok = x == 1;
           }
-          mma_commit(delta_done);
+          if (!ok) break;
           mma_commit(&empty[s]);
-          ok = true;
         }
       }
       mma_commit(drained);
@@ -988,37 +1042,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (!mbar_wait_bounded(&full_v[s], (it >> 1) & 1)) break;
           if (r >= n) zero_v_row<DV>(smem + L::kV + s * L::kVBytes, r, half);
         }
-        // the further parts' buffers are free once the last chunk's D is complete
-        if (it >= 1 && !mbar_wait_bounded(delta_done, (it - 1) & 1)) break;
-        const float w = r < n ? kv_weight(u, r, n, reverse) : 0.0f;
-#pragma unroll
-        for (int q = 0; q < DK / 16; ++q) {
-          const int at = piece_at(r, half * (DK / 16) + q, kC);
-          const uint4 x = *reinterpret_cast<const uint4*>(ks + at);
-          const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-          float f[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 g = unpack2<T>(in[e]);
-            f[2 * e] = r < n ? g.x * w : 0.0f;
-            f[2 * e + 1] = r < n ? g.y * w : 0.0f;
-          }
-#pragma unroll
-          for (int part = 0; part < PARTS; ++part) {
-            uint32_t y[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              y[e] = pack2<T>(f[2 * e], f[2 * e + 1]);
-              const float2 back = unpack2<T>(y[e]);
-              f[2 * e] -= back.x;
-              f[2 * e + 1] -= back.y;
-            }
-            uint8_t* to = part == 0 ? ks : smem + L::kLo + (part - 1) * L::kKBytes;
-            *reinterpret_cast<uint4*>(to + at) = make_uint4(y[0], y[1], y[2], y[3]);
-          }
-        }
+        // the further parts' buffers are free once the last chunk's products are
+        // complete; the two halves of a chunk's steps go through on their own
+        if (it >= 1 && !mbar_wait_bounded(&kw_used[r >> 6], (it - 1) & 1)) break;
+        weigh_k_row<T, DK, PARTS>(ks, smem + L::kLo, r, half,
+                                  r < n ? kv_weight(u, r, n, reverse) : 0.0f, r < n);
         fence_proxy_async_smem();
-        warp_arrive(kw_ready, lane);
+        warp_arrive(&kw_ready[r >> 6], lane);
         ok = true;
       }
     }
@@ -1056,7 +1086,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int i = 0; i < u.chunks; ++i, ++it) {
         const int n = chunk_steps(u, chunk_t0(u, i, reverse));
         ok = false;
-        if (!mbar_wait_bounded(delta_done, it & 1)) break;
+        // (the second half's products come after the first's)
+        if (!mbar_wait_bounded(&kw_used[1], it & 1)) break;
         tc_fence_after();
         if (holds) {
           const float gn = decay_pow(u.log2g, n);
