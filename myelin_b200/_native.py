@@ -10,6 +10,7 @@ missing, or a tensor is not on a CUDA device, the call raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -176,6 +177,23 @@ def require_cuda(tensor: torch.Tensor, what: str = "inputs") -> None:
             f"myelin_b200 runs on CUDA devices only; {what} is on {tensor.device}. "
             "Move the tensors to a CUDA device (there is no CPU fallback)."
         )
+
+
+def _launch(name: str, device: int, *args: object) -> None:
+    """Call C entry ``name`` with ``args`` and the current stream of CUDA device
+    ``device``, made current for the call where it is not, and raise on an error.
+
+    A launch is a few microseconds of host time, so this asks torch's C layer
+    directly instead of entering ``torch.cuda.device`` each time."""
+
+    fn = getattr(lib(), name)
+    if torch._C._cuda_getDevice() == device:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status != 0:
+        check(status, name)
 
 
 def device_status(clear: bool = True) -> int:
@@ -558,21 +576,12 @@ class StepsC(ctypes.Structure):
 
     _fields_ = [("data", _vp), ("stride_t", _i64), ("stride_b", _i64), ("stride_h", _i64)]
 
-    @classmethod
-    def of(cls, t: torch.Tensor) -> "StepsC":
-        st, sb, sh, _ = t.stride()
-        return cls(t.data_ptr(), st, sb, sh)
-
 
 class MemoryC(ctypes.Structure):
     """``mb_memory``: an fp32 [B, H, rows, cols] tensor of any strides."""
 
     _fields_ = [("data", _vp), ("stride_b", _i64), ("stride_h", _i64), ("stride_row", _i64),
                 ("stride_col", _i64)]
-
-    @classmethod
-    def of(cls, t: torch.Tensor | None) -> "MemoryC":
-        return cls() if t is None else cls(t.data_ptr(), *t.stride())
 
 
 class DecayAttentionArgsC(ctypes.Structure):
@@ -594,6 +603,13 @@ class DecayAttentionStepArgsC(ctypes.Structure):
                 ("memory_out", _vp), ("active", _vp), ("scale", _f)]
 
 
+# The same two structures as packed bytes: filling one is a single call, where the
+# ctypes classes set 35 fields one by one.
+_ATTENTION_ARGS = struct.Struct("@ii5q" + "Pqqq" * 4 + "PP" + "Pqqqq" * 2 + "ff")
+_ATTENTION_STEP_ARGS = struct.Struct("@i4q4P6q4Pf0q")
+_NO_MEMORY = (0, 0, 0, 0, 0)
+
+
 def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
                     decay: torch.Tensor, lengths: torch.Tensor | None,
                     first: torch.Tensor | None, last: torch.Tensor | None, *, reverse: bool,
@@ -602,19 +618,19 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.
     ``first`` and ``last`` may have any strides (a transposed view included)."""
 
     T, B, H, Dk = q.shape
-    args = DecayAttentionArgsC(
-        dtype_code(q.dtype), int(reverse), T, B, H, Dk, v.shape[3], StepsC.of(q), StepsC.of(k),
-        StepsC.of(v), StepsC.of(o), ptr(decay), ptr(lengths), MemoryC.of(first),
-        MemoryC.of(last), out_scale, kv_scale,
-    )
-    at = ctypes.addressof(args)
-    with torch.cuda.device(q.device):
-        need = int(lib().mb_decay_attention_workspace_bytes(at))
-        if need < 0:
-            check(1, "mb_decay_attention")
-        ws = torch.empty(need // 4, dtype=torch.float32, device=q.device) if need > 0 else None
-        status = lib().mb_decay_attention(at, ptr(ws), need, stream_handle(q.device))
-    check(status, "mb_decay_attention")
+    args = _ATTENTION_ARGS.pack(
+        _DTYPE_CODES[q.dtype], reverse, T, B, H, Dk, v.shape[3],
+        q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3],
+        v.data_ptr(), *v.stride()[:3], o.data_ptr(), *o.stride()[:3],
+        decay.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+        *(_NO_MEMORY if first is None else (first.data_ptr(), *first.stride())),
+        *(_NO_MEMORY if last is None else (last.data_ptr(), *last.stride())),
+        out_scale, kv_scale)
+    need = lib().mb_decay_attention_workspace_bytes(args)
+    if need < 0:
+        check(1, "mb_decay_attention")
+    ws = torch.empty(need // 4, dtype=torch.float32, device=q.device) if need > 0 else None
+    _launch("mb_decay_attention", q.get_device(), args, ptr(ws), need)
 
 
 def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
@@ -624,35 +640,28 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
     and contiguous memories [B, H, Dk, Dv]."""
 
     B, H, Dk = q.shape
-    args = DecayAttentionStepArgsC(
-        dtype_code(q.dtype), B, H, Dk, v.shape[2], ptr(q), ptr(k), ptr(v), ptr(o), q.stride(0),
-        q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), ptr(decay),
-        ptr(memory_in), ptr(memory_out), ptr(active), scale,
-    )
-    with torch.cuda.device(q.device):
-        status = lib().mb_decay_attention_step(ctypes.addressof(args), stream_handle(q.device))
-    check(status, "mb_decay_attention_step")
+    args = _ATTENTION_STEP_ARGS.pack(
+        _DTYPE_CODES[q.dtype], B, H, Dk, v.shape[2], q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        o.data_ptr(), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], decay.data_ptr(),
+        memory_in.data_ptr(), memory_out.data_ptr(), 0 if active is None else active.data_ptr(),
+        scale)
+    _launch("mb_decay_attention_step", q.get_device(), args)
 
 
 def dropout(x: torch.Tensor, y: torch.Tensor, rows: int, n: int, threshold: int,
             seed: torch.Tensor) -> None:
     """``mb_dropout`` over contiguous ``x[rows, n]``, one mask for all rows."""
 
-    with torch.cuda.device(x.device):
-        status = lib().mb_dropout(dtype_code(x.dtype), ptr(x), ptr(y), rows, n, threshold,
-                                  ptr(seed), stream_handle(x.device))
-    check(status, "mb_dropout")
+    _launch("mb_dropout", x.get_device(), _DTYPE_CODES[x.dtype], x.data_ptr(), y.data_ptr(), rows,
+            n, threshold, seed.data_ptr())
 
 
 def quantize_rows(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
     """``mb_quantize_rows``: int8 ``q[M, K]`` and fp32 ``scale[M]`` of ``x[M, K]``
     (rows contiguous along K, any pitch)."""
 
-    with torch.cuda.device(x.device):
-        status = lib().mb_quantize_rows(dtype_code(x.dtype), ptr(x), x.shape[0], x.shape[1],
-                                        x.stride(0), ptr(q), q.stride(0), ptr(scale),
-                                        stream_handle(x.device))
-    check(status, "mb_quantize_rows")
+    _launch("mb_quantize_rows", x.get_device(), _DTYPE_CODES[x.dtype], x.data_ptr(), x.shape[0],
+            x.shape[1], x.stride(0), q.data_ptr(), q.stride(0), scale.data_ptr())
 
 
 def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor | None, b: torch.Tensor,
@@ -660,14 +669,10 @@ def gemm_i8(a: torch.Tensor, a_scale: torch.Tensor | None, b: torch.Tensor,
     """``mb_gemm_i8``: int8 ``a[M, K]``, ``b[N, K]`` with 16-byte row pitches."""
 
     M, K = a.shape
-    N = b.shape[0]
-    with torch.cuda.device(a.device):
-        status = lib().mb_gemm_i8(
-            ptr(a), a.stride(0), ptr(a_scale), ptr(b), b.stride(0), ptr(b_scale), ptr(bias),
-            dtype_code(bias.dtype) if bias is not None else 0, dtype_code(out.dtype), ptr(out),
-            out.stride(0), M, N, K, stream_handle(a.device),
-        )
-    check(status, "mb_gemm_i8")
+    _launch("mb_gemm_i8", a.get_device(), a.data_ptr(), a.stride(0), ptr(a_scale), b.data_ptr(),
+            b.stride(0), b_scale.data_ptr(), ptr(bias),
+            _DTYPE_CODES[bias.dtype] if bias is not None else 0, _DTYPE_CODES[out.dtype],
+            out.data_ptr(), out.stride(0), M, b.shape[0], K)
 
 
 # mb_linear_i8_rows: rows and staged bytes it takes (mb_linear_i8_rows_supported)
@@ -679,11 +684,7 @@ def linear_i8_rows(x: torch.Tensor, x_scale: torch.Tensor | None, w: torch.Tenso
     """``mb_linear_i8_rows``: a few rows ``x[M, K]`` (float, or int8 / bool) by int8 ``w[N, K]``."""
 
     M, K = x.shape
-    with torch.cuda.device(x.device):
-        status = lib().mb_linear_i8_rows(
-            dtype_code(x.dtype), ptr(x), x.stride(0), ptr(x_scale), ptr(w), w.stride(0),
-            ptr(w_scale), ptr(bias), dtype_code(bias.dtype) if bias is not None else 0,
-            dtype_code(out.dtype), ptr(out), out.stride(0), M, w.shape[0], K,
-            stream_handle(x.device),
-        )
-    check(status, "mb_linear_i8_rows")
+    _launch("mb_linear_i8_rows", x.get_device(), _DTYPE_CODES[x.dtype], x.data_ptr(), x.stride(0),
+            ptr(x_scale), w.data_ptr(), w.stride(0), w_scale.data_ptr(), ptr(bias),
+            _DTYPE_CODES[bias.dtype] if bias is not None else 0, _DTYPE_CODES[out.dtype],
+            out.data_ptr(), out.stride(0), M, w.shape[0], K)

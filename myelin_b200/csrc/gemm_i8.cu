@@ -395,13 +395,25 @@ __device__ __forceinline__ void drain_i8(uint32_t taddr, int64_t row0, int64_t c
       constexpr int W = 32 * kPerStore;
       const int rows = static_cast<int>(imin64(32, args.M - row0));
       TOut* c = static_cast<TOut*>(args.C) + row0 * args.ldc + block0;
-      for (int i = 0; i < rows; ++i) {
+#pragma unroll 1
+      for (int i0 = 0; i0 < rows; i0 += 8) {  // eight rows' reads in flight
+        TOut held[8][W / 32];
 #pragma unroll
-        for (int j = 0; j < W / 32; ++j) {
-          const int e = j * 32 + lane;
-          const int byte = e * int(sizeof(TOut));
-          const int at = i * 128 + (((byte >> 4) ^ (i & 7)) << 4) + (byte & 15);
-          if (block0 + e < args.N) c[i * args.ldc + e] = *reinterpret_cast<const TOut*>(slot + at);
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+          for (int j = 0; j < W / 32; ++j) {
+            const int byte = (j * 32 + lane) * int(sizeof(TOut));
+            const int at = (i0 + i) * 128 + (((byte >> 4) ^ i) << 4) + (byte & 15);
+            held[i][j] = *reinterpret_cast<const TOut*>(slot + at);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+          for (int j = 0; j < W / 32; ++j) {
+            const int e = j * 32 + lane;
+            if (i0 + i < rows && block0 + e < args.N) c[(i0 + i) * args.ldc + e] = held[i][j];
+          }
         }
       }
     }

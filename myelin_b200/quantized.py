@@ -139,11 +139,11 @@ def quantized_linear(
         out_dtype = x.dtype if x.dtype.is_floating_point else torch.float32
     if out_dtype not in nat.SCAN_DTYPES:
         raise ValueError(f"out_dtype must be float32, bfloat16 or float16; got {out_dtype}")
-    if torch.is_grad_enabled() and (x.requires_grad or weight.scale.requires_grad
-                                    or (bias is not None and bias.requires_grad)):
+    if (x.requires_grad or weight.scale.requires_grad
+            or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
         raise NotImplementedError("quantized_linear is forward only; detach its inputs or call "
                                   "it under torch.no_grad()")
     out = cops.quantized_project(
-        x.reshape(-1, K), None if scale is None else scale.reshape(-1).contiguous(), weight.data,
+        x if x.ndim == 2 else x.reshape(-1, K), None if scale is None else scale.reshape(-1).contiguous(), weight.data,
         weight.scale.contiguous(), None if bias is None else bias.contiguous(), out_dtype)
-    return out.view(*x.shape[:-1], N)
+    return out if x.ndim == 2 else out.view(*x.shape[:-1], N)

@@ -135,6 +135,20 @@ def test_c_entry_reports_bad_arguments(kw, message):
     assert re.search(message, lib.mb_last_error().decode())
 
 
+def test_packed_arguments_have_the_structures_layout():
+    for packed, c in ((nat._ATTENTION_ARGS, nat.DecayAttentionArgsC),
+                      (nat._ATTENTION_STEP_ARGS, nat.DecayAttentionStepArgsC)):
+        assert packed.size == ctypes.sizeof(c)
+    values = list(range(1, 36)) + [0.5, 0.25]
+    a = nat.DecayAttentionArgsC.from_buffer_copy(nat._ATTENTION_ARGS.pack(*values))
+    assert (a.dtype, a.reverse, a.T, a.Dv, a.q.data) == (1, 2, 3, 7, 8)
+    assert (a.k.stride_t, a.o.stride_h, a.decay, a.lengths) == (13, 23, 24, 25)
+    assert (a.first.data, a.last.stride_col, a.out_scale, a.kv_scale) == (26, 35, 0.5, 0.25)
+    values = list(range(1, 20)) + [0.5]
+    b = nat.DecayAttentionStepArgsC.from_buffer_copy(nat._ATTENTION_STEP_ARGS.pack(*values))
+    assert [getattr(b, name) for name, _ in b._fields_] == values
+
+
 def test_c_entry_empty_and_workspace():
     lib = nat.lib()
     assert lib.mb_decay_attention(ctypes.addressof(_args(B=0)), None, 0, None) == 0
