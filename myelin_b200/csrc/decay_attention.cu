@@ -14,23 +14,43 @@ constexpr int kRecWarps = kRecThreads / 32;
 __host__ __device__ constexpr int rec_steps(int rows) { return rows >= 32 ? 8 : 16; }
 
 // ---------------------------------------------------------------------------
-// Recurrent kernel: any head size up to 256, any element type and stride, sums
-// in fp32 in the order of the recurrence. A block holds 32 columns of one
-// memory in registers (lane = column, each warp R of the Dk rows), stages a few
-// steps of q, k and v in shared memory as fp32, walks them without a barrier
-// and then adds the eight warps' partial outputs. Three fp32 instructions per
-// memory element and step bound it (about 3 Dk Dv per step and head).
+// Recurrent kernel: any head size up to 256, any element type and stride, sums in
+// fp32. A block holds 32 columns of one memory in registers (lane = column, each
+// warp R of the Dk rows), stages TC steps of q, k and v in shared memory as fp32
+// (the next ones on their way meanwhile), walks them without a barrier and then adds
+// the eight warps' partial outputs.
+//
+// The leak is taken out of the inner loop: over a burst of steps p = 0, 1, ... the
+// block keeps g^-p S_p, so that a step is two FMAs per memory element (in pairs,
+// f32x2) instead of a product and two FMAs:
+//   S~ += (g^-p k_p) v_p^T,   o_p = g^p q_p^T S~,
+// with the leak of the first step applied before a forward burst, that of the last
+// one after a reverse burst. The powers are formed in double, so that g^-p g^p is 1
+// to two roundings. Decays below 0.02 (whose powers would leave fp32's range) take
+// bursts of one step. About 2 Dk Dv FMAs per step and head bound it.
 // ---------------------------------------------------------------------------
+__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
+        "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
 template <typename T, int R, bool STATES_ONLY>
 __global__ void __launch_bounds__(kRecThreads)
     attn_recurrent_kernel(const __grid_constant__ mb_decay_attention_args a,
                           const __grid_constant__ AttnSplit split) {
   constexpr int TC = rec_steps(R);
   constexpr int ROWS = R * kRecWarps;
+  constexpr int NK = TC * ROWS / kRecThreads;               // staged k (q) elements per thread
+  constexpr int NV = (TC * kCols + kRecThreads - 1) / kRecThreads;
   __shared__ __align__(16) float sk[TC][ROWS];
   __shared__ __align__(16) float sq[STATES_ONLY ? 1 : TC][ROWS];
   __shared__ float sv[TC][kCols];
   __shared__ float part[STATES_ONLY ? 1 : TC][kRecWarps][kCols];
+  __shared__ float s_pow[TC + 1], s_inv[TC];  // g^p, g^-p
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t tiles = (a.Dv + kCols - 1) / kCols;
@@ -57,68 +77,95 @@ __global__ void __launch_bounds__(kRecThreads)
   T* o = static_cast<T*>(a.o.data) + b * a.o.stride_b + h * a.o.stride_h;
   const float g = a.decay[h];
   const bool reverse = a.reverse != 0;
+  const int burst = g >= 0.02f ? TC : 1;
+  if (threadIdx.x <= TC) {
+    double p = 1.0;
+    for (int i = 0; i < int(threadIdx.x); ++i) p *= static_cast<double>(g);
+    s_pow[threadIdx.x] = static_cast<float>(p);
+    if (threadIdx.x < TC) s_inv[threadIdx.x] = burst == 1 ? 1.0f : static_cast<float>(1.0 / p);
+  }
 
-  float S[R];
+  float2 S[R / 2];
   const int64_t seg_at = ((seg * a.B + b) * a.H + h) * a.Dk;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int64_t r = row0 + i;
-    S[i] = 0.0f;
-    if (!col_ok || r >= a.Dk || STATES_ONLY) continue;
-    if (split.segments > 1) {
-      S[i] = split.states[(seg_at + r) * a.Dv + col];
-    } else if (a.first.data != nullptr) {
-      S[i] = a.first.data[b * a.first.stride_b + h * a.first.stride_h + r * a.first.stride_row +
-                          col * a.first.stride_col];
+    float x = 0.0f;
+    if (col_ok && r < a.Dk && !STATES_ONLY) {
+      if (split.segments > 1) {
+        x = split.states[(seg_at + r) * a.Dv + col];
+      } else if (a.first.data != nullptr) {
+        x = a.first.data[b * a.first.stride_b + h * a.first.stride_h + r * a.first.stride_row +
+                         col * a.first.stride_col];
+      }
     }
+    (i & 1 ? S[i / 2].y : S[i / 2].x) = x;
   }
 
+  // this thread's elements of the next steps' k, q and v
+  float rk[NK], rq[STATES_ONLY ? 1 : NK], rv[NV];
+  auto step_at = [&](int64_t p) { return reverse ? end - 1 - p : lo + p; };
+  auto fetch = [&](int64_t p0) {
+    const int steps = static_cast<int>(imin64(TC, n - p0));
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const int e = threadIdx.x + i * kRecThreads, s = e / ROWS, d = e % ROWS;
+      const bool ok = s < steps && d < a.Dk;
+      const int64_t t = step_at(p0 + s);
+      rk[i] = ok ? Elem<T>::to_f(k[t * a.k.stride_t + d]) : 0.0f;
+      if constexpr (!STATES_ONLY) rq[i] = ok ? Elem<T>::to_f(q[t * a.q.stride_t + d]) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = threadIdx.x + i * kRecThreads, s = e / kCols, c = e % kCols;
+      rv[i] = s < steps && col0 + c < a.Dv
+                  ? Elem<T>::to_f(v[step_at(p0 + s) * a.v.stride_t + col0 + c])
+                  : 0.0f;
+    }
+  };
+  auto scale_memory = [&](float w) {
+    const float2 w2 = make_float2(w, w), zero = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < R / 2; ++i) S[i] = fma_pair(S[i], w2, zero);
+  };
+  if (n > 0) fetch(0);
   for (int64_t p0 = 0; p0 < n; p0 += TC) {
     const int steps = static_cast<int>(imin64(TC, n - p0));
-    __syncthreads();  // the previous steps' staging has been read
-    for (int e = threadIdx.x; e < TC * ROWS; e += kRecThreads) {
-      const int s = e / ROWS, d = e % ROWS;
-      const int64_t t = reverse ? end - 1 - (p0 + s) : lo + p0 + s;
-      const bool ok = s < steps && d < a.Dk;
-      sk[s][d] = ok ? Elem<T>::to_f(k[t * a.k.stride_t + d]) * a.kv_scale : 0.0f;
-      if constexpr (!STATES_ONLY) {
-        sq[s][d] = ok ? Elem<T>::to_f(q[t * a.q.stride_t + d]) : 0.0f;
-      }
+    __syncthreads();  // the previous steps' staging has been read; the powers are written
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const int e = threadIdx.x + i * kRecThreads, s = e / ROWS;
+      sk[s][e % ROWS] = rk[i] * (a.kv_scale * s_inv[s]);
+      if constexpr (!STATES_ONLY) sq[s][e % ROWS] = rq[i];
     }
-    for (int e = threadIdx.x; e < TC * kCols; e += kRecThreads) {
-      const int s = e / kCols, c = e % kCols;
-      const int64_t t = reverse ? end - 1 - (p0 + s) : lo + p0 + s;
-      sv[s][c] = s < steps && col0 + c < a.Dv ? Elem<T>::to_f(v[t * a.v.stride_t + col0 + c])
-                                              : 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = threadIdx.x + i * kRecThreads;
+      if (e < TC * kCols) sv[e / kCols][e % kCols] = rv[i];
     }
     __syncthreads();
-    for (int s = 0; s < steps; ++s) {
-      const float vc = sv[s][lane];
-      float acc = 0.0f;
+    if (p0 + TC < n) fetch(p0 + TC);
+    for (int s0 = 0; s0 < steps; s0 += burst) {
+      const int s1 = min(steps, s0 + burst);
+      if (!reverse) scale_memory(g);
+#pragma unroll 2
+      for (int s = s0; s < s1; ++s) {
+        const float2 vc = make_float2(sv[s][lane], sv[s][lane]);
+        float2 acc = make_float2(0.0f, 0.0f), acc2 = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int i = 0; i < R; i += 4) {
-        const float4 kk = *reinterpret_cast<const float4*>(&sk[s][row0 + i]);
-        const float ks[4] = {kk.x, kk.y, kk.z, kk.w};
-        if (reverse) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[i + e] = fmaf(ks[e], vc, S[i + e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[i + e] = fmaf(g, S[i + e], ks[e] * vc);
+        for (int i = 0; i < R; i += 4) {
+          const float4 kk = *reinterpret_cast<const float4*>(&sk[s][row0 + i]);
+          S[i / 2] = fma_pair(make_float2(kk.x, kk.y), vc, S[i / 2]);
+          S[i / 2 + 1] = fma_pair(make_float2(kk.z, kk.w), vc, S[i / 2 + 1]);
+          if constexpr (!STATES_ONLY) {
+            const float4 qq = *reinterpret_cast<const float4*>(&sq[s][row0 + i]);
+            acc = fma_pair(make_float2(qq.x, qq.y), S[i / 2], acc);
+            acc2 = fma_pair(make_float2(qq.z, qq.w), S[i / 2 + 1], acc2);
+          }
         }
-        if constexpr (!STATES_ONLY) {
-          const float4 qq = *reinterpret_cast<const float4*>(&sq[s][row0 + i]);
-          acc = fmaf(qq.x, S[i], acc);
-          acc = fmaf(qq.y, S[i + 1], acc);
-          acc = fmaf(qq.z, S[i + 2], acc);
-          acc = fmaf(qq.w, S[i + 3], acc);
-        }
-        if (reverse) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[i + e] *= g;
-        }
+        if constexpr (!STATES_ONLY) part[s][warp][lane] = (acc.x + acc.y) + (acc2.x + acc2.y);
       }
-      if constexpr (!STATES_ONLY) part[s][warp][lane] = acc;
+      scale_memory(s_pow[reverse ? s1 - s0 : s1 - s0 - 1]);
     }
     if constexpr (!STATES_ONLY) {
       __syncthreads();
@@ -128,8 +175,8 @@ __global__ void __launch_bounds__(kRecThreads)
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kRecWarps; ++w) sum += part[s][w][c];
-        const int64_t t = reverse ? end - 1 - (p0 + s) : lo + p0 + s;
-        o[t * a.o.stride_t + col0 + c] = Elem<T>::from_f(sum * a.out_scale);
+        const float out = burst == 1 ? a.out_scale : a.out_scale * s_pow[s];
+        o[step_at(p0 + s) * a.o.stride_t + col0 + c] = Elem<T>::from_f(sum * out);
       }
     }
   }
@@ -142,19 +189,17 @@ __global__ void __launch_bounds__(kRecThreads)
     }
   }
   if (!col_ok) return;
-  if constexpr (STATES_ONLY) {
+  const bool whole = !STATES_ONLY && split.segments == 1 && a.last.data != nullptr;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      if (row0 + i < a.Dk) split.states[(seg_at + row0 + i) * a.Dv + col] = S[i];
-    }
-  } else if (split.segments == 1 && a.last.data != nullptr) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int64_t r = row0 + i;
-      if (r < a.Dk) {
-        a.last.data[b * a.last.stride_b + h * a.last.stride_h + r * a.last.stride_row +
-                    col * a.last.stride_col] = S[i];
-      }
+  for (int i = 0; i < R; ++i) {
+    const int64_t r = row0 + i;
+    const float x = i & 1 ? S[i / 2].y : S[i / 2].x;
+    if (r >= a.Dk) continue;
+    if constexpr (STATES_ONLY) {
+      split.states[(seg_at + r) * a.Dv + col] = x;
+    } else if (whole) {
+      a.last.data[b * a.last.stride_b + h * a.last.stride_h + r * a.last.stride_row +
+                  col * a.last.stride_col] = x;
     }
   }
 }

@@ -43,106 +43,151 @@ __device__ __forceinline__ RowScale row_scale(float top) {
   return RowScale{__fdiv_rn(127.0f, top), __fdiv_rn(top, 127.0f)};
 }
 
-// max that keeps a NaN (fmaxf would drop it)
-__device__ __forceinline__ float max_nan(float a, float b) {
-  return (b > a || b != b) ? b : a;
+// Magnitudes as bit patterns: ordered like the numbers, with NaN above infinity, so
+// that an integer maximum keeps a NaN (fmaxf would drop it).
+__device__ __forceinline__ uint32_t top_of(uint32_t top, float x) {
+  return max(top, __float_as_uint(x) & 0x7fffffffu);
 }
 
+// Eight (fewer) values times inv, rounded to integers, as bytes. Adding 1.5 * 2^23
+// rounds to the nearest integer (ties to even) and leaves it in the low bits; the
+// product is rounded on its own first, as the definition has it. |x| inv is at most
+// 127 (1 + 2^-22). A row with inv = 0 is zero whatever it holds.
+__device__ __forceinline__ uint32_t quantize_bits(float x, float inv) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f));
+}
 __device__ __forceinline__ int8_t quantize(float x, float inv) {
-  // |x| * inv is at most 127 (1 + 2^-22); inv = 0 sends 0 * inf's NaN to 0
-  return static_cast<int8_t>(inv == 0.0f ? 0 : __float2int_rn(__fmul_rn(x, inv)));
+  return inv == 0.0f ? int8_t(0) : static_cast<int8_t>(quantize_bits(x, inv) & 0xffu);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t quantize4(const T* v, float inv) {
+  if (inv == 0.0f) return 0u;
+  const uint32_t a = quantize_bits(Elem<T>::to_f(v[0]), inv);
+  const uint32_t b = quantize_bits(Elem<T>::to_f(v[1]), inv);
+  const uint32_t c = quantize_bits(Elem<T>::to_f(v[2]), inv);
+  const uint32_t d = quantize_bits(Elem<T>::to_f(v[3]), inv);
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// TPR threads per row. Aligned rows of up to TPR * 8 * kHold elements stay in
-// registers between the two passes; longer or unaligned ones are read twice.
-constexpr int kHold = 4;
+// Largest magnitude of one 16-byte piece, joined with `top`: the bits of one fp32, or
+// of two 16-bit values side by side (each half its own maximum).
+template <typename T>
+__device__ __forceinline__ uint32_t piece_top(uint32_t top, const uint4& x) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    top = sizeof(T) == 2 ? __vmaxu2(top, w[i] & 0x7fff7fffu) : max(top, w[i] & 0x7fffffffu);
+  }
+  return top;
+}
 
-template <typename T, int TPR, bool VECTOR>
+// The maximum that piece_top gathered, as an fp32 value's bits.
+template <typename T>
+__device__ __forceinline__ uint32_t whole_top(uint32_t top) {
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t half = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
+    return __float_as_uint(Elem<T>::to_f(*reinterpret_cast<const T*>(&half)));
+  } else {
+    return top;
+  }
+}
+
+// A piece quantised: 8 bytes of a 16-bit type's values, 4 of fp32's.
+template <typename T>
+__device__ __forceinline__ void put_piece(int8_t* q, const uint4& x, float inv) {
+  const T* v = reinterpret_cast<const T*>(&x);
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint2*>(q) = make_uint2(quantize4<T>(v, inv), quantize4<T>(v + 4, inv));
+  } else {
+    *reinterpret_cast<uint32_t*>(q) = quantize4<T>(v, inv);
+  }
+}
+
+// TPR threads per row, HOLD 16-byte pieces of it in registers between the two passes
+// (all on their way at once); what is longer, or not aligned, is read twice. Bound by
+// DRAM: 3 bytes per 16-bit value (5 per fp32). A warp that holds a whole row needs no
+// barrier; a block per row of 4096 columns reached 2.8 TB/s.
+template <typename T, int TPR, int HOLD>
 __global__ void __launch_bounds__(256)
-    quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t ldx,
+    quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx,
                          int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
-  using V = Vec<T, 8>;
   constexpr int RPB = 256 / TPR;
-  __shared__ float tops[8];
+  constexpr int E = 16 / sizeof(T);
+  __shared__ uint32_t tops[8];
   const int t = threadIdx.x % TPR;
   const int64_t row = int64_t(blockIdx.x) * RPB + threadIdx.x / TPR;
   const bool ok = row < rows;
   const T* xr = x + row * ldx;
   int8_t* qr = q + row * ldq;
-  float top = 0.0f;
-  V held[kHold];
-  if (ok) {
-    if constexpr (VECTOR) {
+  uint32_t top = 0;
+  uint4 held[HOLD > 0 ? HOLD : 1];
+  const int pieces = HOLD > 0 && ok ? cols / E : 0;
+  const uint4* xp = reinterpret_cast<const uint4*>(xr);
+  if constexpr (HOLD > 0) {
 #pragma unroll
-      for (int i = 0; i < kHold; ++i) {
-        const int64_t c = (int64_t(i) * TPR + t) * 8;
-        if (c < cols) {
-          held[i] = load_vec<T, 8>(xr + c);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(Elem<T>::to_f(held[i].v[j])));
-        }
-      }
-      for (int64_t c = (int64_t(kHold) * TPR + t) * 8; c < cols; c += TPR * 8) {
-        const V v = load_vec<T, 8>(xr + c);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(Elem<T>::to_f(v.v[j])));
-      }
-    } else {
-      for (int64_t c = t; c < cols; c += TPR) top = max_nan(top, fabsf(Elem<T>::to_f(xr[c])));
+    for (int i = 0; i < HOLD; ++i) {
+      if (i * TPR + t < pieces) held[i] = xp[i * TPR + t];
     }
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+      if (i * TPR + t < pieces) top = piece_top<T>(top, held[i]);
+    }
+    for (int p = HOLD * TPR + t; p < pieces; p += TPR) top = piece_top<T>(top, xp[p]);
+    top = whole_top<T>(top);
+  } else if (ok) {
+    for (int c = t; c < cols; c += TPR) top = top_of(top, Elem<T>::to_f(xr[c]));
   }
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+  for (int d = 16; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
   if constexpr (TPR > 32) {
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
     __syncthreads();
     top = tops[0];
 #pragma unroll
-    for (int w = 1; w < TPR / 32; ++w) top = max_nan(top, tops[w]);
+    for (int w = 1; w < TPR / 32; ++w) top = max(top, tops[w]);
   }
   if (!ok) return;
-  const RowScale rs = row_scale(top);
+  const RowScale rs = row_scale(__uint_as_float(top));
   if (t == 0) scale[row] = rs.scale;
-  if constexpr (VECTOR) {
-    auto put = [&](const V& v, int64_t c) {
-      Vec<int8_t, 8> o;
+  if constexpr (HOLD > 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o.v[j] = quantize(Elem<T>::to_f(v.v[j]), rs.inv);
-      store_vec<int8_t, 8>(qr + c, o);
-    };
-#pragma unroll
-    for (int i = 0; i < kHold; ++i) {
-      const int64_t c = (int64_t(i) * TPR + t) * 8;
-      if (c < cols) put(held[i], c);
+    for (int i = 0; i < HOLD; ++i) {
+      const int p = i * TPR + t;
+      if (p < pieces) put_piece<T>(qr + p * E, held[i], rs.inv);
     }
-    for (int64_t c = (int64_t(kHold) * TPR + t) * 8; c < cols; c += TPR * 8) {
-      put(load_vec<T, 8>(xr + c), c);
-    }
+    for (int p = HOLD * TPR + t; p < pieces; p += TPR) put_piece<T>(qr + p * E, xp[p], rs.inv);
   } else {
-    for (int64_t c = t; c < cols; c += TPR) qr[c] = quantize(Elem<T>::to_f(xr[c]), rs.inv);
+    for (int c = t; c < cols; c += TPR) qr[c] = quantize(Elem<T>::to_f(xr[c]), rs.inv);
   }
 }
 
+template <typename T, int TPR, int HOLD>
+int launch_quantize_as(const T* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq,
+                       float* scale, cudaStream_t s) {
+  const int64_t blocks = ceil_div(rows, 256 / TPR);
+  MB_CHECK_ARG(blocks <= 0x7fffffff, "mb_quantize_rows: too many rows");
+  quantize_rows_kernel<T, TPR, HOLD><<<static_cast<unsigned>(blocks), 256, 0, s>>>(
+      x, rows, static_cast<int>(cols), ldx, q, ldq, scale);
+  MB_CHECK_LAUNCH("mb_quantize_rows");
+  return 0;
+}
+
+// A warp per row while the row fits its registers, else the whole block.
 template <typename T>
 int launch_quantize(const void* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* q,
                     int64_t ldq, float* scale, cudaStream_t s) {
+  constexpr int E = 16 / sizeof(T);
   const T* xs = static_cast<const T*>(x);
-  const bool vector = cols % 8 == 0 && aligned_to(x, 16) && (ldx * int64_t(sizeof(T))) % 16 == 0 &&
-                      aligned_to(q, 8) && ldq % 8 == 0;
-  // a warp per row while a row fits its registers, else the whole block
-  const bool narrow = cols <= 32 * 8 * kHold;
-  const int64_t blocks = narrow ? ceil_div(rows, 8) : rows;
-  MB_CHECK_ARG(blocks <= 0x7fffffff, "mb_quantize_rows: too many rows");
-  const unsigned grid = static_cast<unsigned>(blocks);
-  if (narrow) {
-    if (vector) quantize_rows_kernel<T, 32, true><<<grid, 256, 0, s>>>(xs, rows, cols, ldx, q, ldq, scale);
-    else quantize_rows_kernel<T, 32, false><<<grid, 256, 0, s>>>(xs, rows, cols, ldx, q, ldq, scale);
-  } else {
-    if (vector) quantize_rows_kernel<T, 256, true><<<grid, 256, 0, s>>>(xs, rows, cols, ldx, q, ldq, scale);
-    else quantize_rows_kernel<T, 256, false><<<grid, 256, 0, s>>>(xs, rows, cols, ldx, q, ldq, scale);
+  const bool vector = cols % E == 0 && aligned_to(x, 16) && ldx % E == 0 && aligned_to(q, 8) &&
+                      ldq % 8 == 0;
+  const int64_t pieces = cols / E;
+  if (!vector) {
+    return cols <= 1024 ? launch_quantize_as<T, 32, 0>(xs, rows, cols, ldx, q, ldq, scale, s)
+                        : launch_quantize_as<T, 256, 0>(xs, rows, cols, ldx, q, ldq, scale, s);
   }
-  MB_CHECK_LAUNCH("mb_quantize_rows");
-  return 0;
+  if (pieces <= 4 * 32) return launch_quantize_as<T, 32, 4>(xs, rows, cols, ldx, q, ldq, scale, s);
+  if (pieces <= 16 * 32) return launch_quantize_as<T, 32, 16>(xs, rows, cols, ldx, q, ldq, scale, s);
+  return launch_quantize_as<T, 256, 4>(xs, rows, cols, ldx, q, ldq, scale, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -190,26 +235,41 @@ __global__ void __launch_bounds__(kRowsThreads)
     linear_i8_rows_kernel(const X* __restrict__ x, int64_t ldx, const int8_t* __restrict__ w,
                           int64_t ldw, const __grid_constant__ I8Args args) {
   extern __shared__ __align__(16) int8_t sx[];  // [M][K rounded up to 16]
-  __shared__ float tops[M][kRowsThreads / 32];
+  __shared__ uint32_t tops[M][kRowsThreads / 32];
   __shared__ float sscale[M];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t n = int64_t(blockIdx.x) * (kRowsThreads / 32) + warp;
+  constexpr int kWarps = kRowsThreads / 32;
   const int64_t K = args.K, Kp = (K + 15) / 16 * 16;
   const int64_t pieces = K / 16;
-  const bool ok = n < args.N;
-  const int8_t* wr = w + n * ldw;
+  int64_t n = int64_t(blockIdx.x) * kWarps + warp;  // this warp's channels: every gridDim * 8th
 
   int4 held[kRowsVecs];
+  auto fetch = [&](int64_t channel) {  // the first pieces of a weight row
+    const int8_t* wr = w + channel * ldw;
 #pragma unroll
-  for (int i = 0; i < kRowsVecs; ++i) {
-    const int64_t p = int64_t(i) * 32 + lane;
-    if (ok && p < pieces) held[i] = __ldg(reinterpret_cast<const int4*>(wr) + p);
-  }
+    for (int i = 0; i < kRowsVecs; ++i) {
+      const int64_t p = int64_t(i) * 32 + lane;
+      if (channel < args.N && p < pieces) held[i] = __ldg(reinterpret_cast<const int4*>(wr) + p);
+    }
+  };
+  fetch(n);
 
   if constexpr (sizeof(X) == 1) {
-    for (int64_t e = threadIdx.x; e < M * Kp; e += kRowsThreads) {
-      const int64_t m = e / Kp, c = e % Kp;
-      sx[e] = c < K ? static_cast<int8_t>(x[m * ldx + c]) : int8_t(0);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const X* xr = x + m * ldx;
+      if ((reinterpret_cast<uintptr_t>(xr) & 15) == 0) {
+        for (int64_t p = threadIdx.x; p < pieces; p += kRowsThreads) {
+          *reinterpret_cast<int4*>(sx + m * Kp + p * 16) = *reinterpret_cast<const int4*>(xr + p * 16);
+        }
+        for (int64_t c = pieces * 16 + threadIdx.x; c < Kp; c += kRowsThreads) {
+          sx[m * Kp + c] = c < K ? static_cast<int8_t>(xr[c]) : int8_t(0);
+        }
+      } else {
+        for (int64_t c = threadIdx.x; c < Kp; c += kRowsThreads) {
+          sx[m * Kp + c] = c < K ? static_cast<int8_t>(xr[c]) : int8_t(0);
+        }
+      }
     }
     if (threadIdx.x < M) {
       sscale[threadIdx.x] = args.a_scale != nullptr ? args.a_scale[threadIdx.x] : 1.0f;
@@ -219,43 +279,43 @@ __global__ void __launch_bounds__(kRowsThreads)
     constexpr int E = 16 / sizeof(X);
     using V = Vec<X, E>;
     const bool vector = K % E == 0 && ldx % E == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-    float top[M];
+    uint32_t top[M];
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      top[m] = 0.0f;
+      top[m] = 0;
       if (vector) {
         for (int64_t c = int64_t(threadIdx.x) * E; c < K; c += kRowsThreads * E) {
           const V v = load_vec<X, E>(x + m * ldx + c);
 #pragma unroll
-          for (int j = 0; j < E; ++j) top[m] = max_nan(top[m], fabsf(Elem<X>::to_f(v.v[j])));
+          for (int j = 0; j < E; ++j) top[m] = top_of(top[m], Elem<X>::to_f(v.v[j]));
         }
       } else {
         for (int64_t c = threadIdx.x; c < K; c += kRowsThreads) {
-          top[m] = max_nan(top[m], fabsf(Elem<X>::to_f(x[m * ldx + c])));
+          top[m] = top_of(top[m], Elem<X>::to_f(x[m * ldx + c]));
         }
       }
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) {
-        top[m] = max_nan(top[m], __shfl_xor_sync(0xffffffffu, top[m], d));
+        top[m] = max(top[m], __shfl_xor_sync(0xffffffffu, top[m], d));
       }
       if (lane == 0) tops[m][warp] = top[m];
     }
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      float t = tops[m][0];
+      uint32_t t = tops[m][0];
 #pragma unroll
-      for (int i = 1; i < kRowsThreads / 32; ++i) t = max_nan(t, tops[m][i]);
-      const RowScale rs = row_scale(t);
+      for (int i = 1; i < kWarps; ++i) t = max(t, tops[m][i]);
+      const RowScale rs = row_scale(__uint_as_float(t));
       if (threadIdx.x == 0) sscale[m] = rs.scale;
       // the row again, from L1 or L2
       if (vector) {
         for (int64_t c = int64_t(threadIdx.x) * E; c < K; c += kRowsThreads * E) {
           const V v = load_vec<X, E>(x + m * ldx + c);
-          Vec<int8_t, E> o;
 #pragma unroll
-          for (int j = 0; j < E; ++j) o.v[j] = quantize(Elem<X>::to_f(v.v[j]), rs.inv);
-          store_vec<int8_t, E>(sx + m * Kp + c, o);
+          for (int j = 0; j < E; j += 4) {
+            *reinterpret_cast<uint32_t*>(sx + m * Kp + c + j) = quantize4<X>(v.v + j, rs.inv);
+          }
         }
         for (int64_t c = K + threadIdx.x; c < Kp; c += kRowsThreads) sx[m * Kp + c] = 0;
       } else {
@@ -266,49 +326,47 @@ __global__ void __launch_bounds__(kRowsThreads)
     }
     __syncthreads();
   }
-  if (!ok) return;
-
-  int acc[M];
+  for (; n < args.N; n += int64_t(gridDim.x) * kWarps) {
+    const int8_t* wr = w + n * ldw;
+    int acc[M];
 #pragma unroll
-  for (int m = 0; m < M; ++m) acc[m] = 0;
-  auto dot = [&](const int4& b, int64_t p) {
+    for (int m = 0; m < M; ++m) acc[m] = 0;
+    for (int64_t p0 = 0; p0 < pieces; p0 += kRowsVecs * 32) {
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      const int4 a = *reinterpret_cast<const int4*>(sx + m * Kp + p * 16);
-      acc[m] = __dp4a(a.x, b.x, acc[m]);
-      acc[m] = __dp4a(a.y, b.y, acc[m]);
-      acc[m] = __dp4a(a.z, b.z, acc[m]);
-      acc[m] = __dp4a(a.w, b.w, acc[m]);
-    }
-  };
-  for (int64_t p0 = 0; p0 < pieces; p0 += kRowsVecs * 32) {
-#pragma unroll
-    for (int i = 0; i < kRowsVecs; ++i) {
-      const int64_t p = p0 + i * 32 + lane;
-      if (p < pieces) {
+      for (int i = 0; i < kRowsVecs; ++i) {
+        const int64_t p = p0 + i * 32 + lane;
+        if (p >= pieces) continue;
         const int4 b = held[i];
         const int64_t ahead = p + kRowsVecs * 32;
         if (ahead < pieces) held[i] = __ldg(reinterpret_cast<const int4*>(wr) + ahead);
-        dot(b, p);
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const int4 a = *reinterpret_cast<const int4*>(sx + m * Kp + p * 16);
+          acc[m] = __dp4a(a.x, b.x, acc[m]);
+          acc[m] = __dp4a(a.y, b.y, acc[m]);
+          acc[m] = __dp4a(a.z, b.z, acc[m]);
+          acc[m] = __dp4a(a.w, b.w, acc[m]);
+        }
       }
     }
-  }
-  const int64_t c = pieces * 16 + lane;  // the row's last K % 16 bytes, one per lane
-  if (c < K) {
+    const int64_t c = pieces * 16 + lane;  // the row's last K % 16 bytes, one per lane
+    if (c < K) {
 #pragma unroll
-    for (int m = 0; m < M; ++m) acc[m] += int(sx[m * Kp + c]) * int(wr[c]);
-  }
-#pragma unroll
-  for (int m = 0; m < M; ++m) {
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], d);
-  }
-  if (lane == 0) {
-    const float sb = args.b_scale[n], bias = load_bias(args, n);
+      for (int m = 0; m < M; ++m) acc[m] += int(sx[m * Kp + c]) * int(wr[c]);
+    }
+    fetch(n + int64_t(gridDim.x) * kWarps);
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      static_cast<TOut*>(args.C)[m * args.ldc + n] =
-          Elem<TOut>::from_f(scaled(acc[m], sscale[m], sb, bias));
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], d);
+    }
+    if (lane == 0) {
+      const float sb = args.b_scale[n], bias = load_bias(args, n);
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        static_cast<TOut*>(args.C)[m * args.ldc + n] =
+            Elem<TOut>::from_f(scaled(acc[m], sscale[m], sb, bias));
+      }
     }
   }
 }
@@ -853,9 +911,9 @@ int launch_gemm_i8(const int8_t* A, int64_t lda, const int8_t* B, int64_t ldb, I
 template <typename X, typename TOut>
 int launch_rows(const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const I8Args& a,
                 cudaStream_t s) {
-  const int64_t blocks = ceil_div(a.N, kRowsThreads / 32);
-  MB_CHECK_ARG(blocks <= 0x7fffffff, "mb_linear_i8_rows: too many output channels");
-  const unsigned grid = static_cast<unsigned>(blocks);
+  // at most three blocks per SM: each stages the input rows once for all its channels
+  const unsigned grid = static_cast<unsigned>(
+      imin64(ceil_div(a.N, kRowsThreads / 32), int64_t(i8_sm_count()) * 3));
   const size_t smem = static_cast<size_t>(a.M * ((a.K + 15) / 16 * 16));
   const X* xs = static_cast<const X*>(x);
   switch (a.M) {
@@ -919,7 +977,8 @@ extern "C" int mb_quantize_rows(int dtype, const void* x, int64_t rows, int64_t 
                                 int8_t* q, int64_t ldq, float* scale, void* stream) {
   using namespace mb;
   clear_error();
-  MB_CHECK_ARG(rows >= 0 && cols >= 1, "mb_quantize_rows: rows must be >= 0 and cols >= 1");
+  MB_CHECK_ARG(rows >= 0 && cols >= 1 && cols < (int64_t(1) << 30),
+               "mb_quantize_rows: rows must be >= 0 and cols >= 1 and below 2^30");
   MB_CHECK_ARG(float_dtype(dtype), "mb_quantize_rows: unsupported dtype %d", dtype);
   if (rows == 0) return 0;
   MB_CHECK_ARG(x != nullptr && q != nullptr && scale != nullptr, "mb_quantize_rows: null tensor");
