@@ -12,8 +12,8 @@
 //
 // All products are tcgen05 (M = 128 steps or memory rows, sums in TMEM). 20 warps:
 //   warp 0      copies: Q, K, V, two stages of 128-byte-swizzled tiles
-//   warp 1      issues the products, one thread: Q S, (W_kv K)^T V, P V, then the next
-//               chunk's Q K^T
+//   warp 1      issues the products, one thread: the next chunk's Q K^T, then this one's
+//               Q S, (W_kv K)^T V and P V
 //   warps 4-11  K -> W_kv K in place, then scores -> P (16 bits, back into TMEM as an
 //               A operand); two warps per 32 rows, half of the columns each
 //   warps 12-19 outputs; the carry in fp32 registers (row per lane, half of the
@@ -75,11 +75,12 @@ struct OutLayout {
   static constexpr int kNumBars = 20;
   static constexpr size_t kSmem = kBars + kNumBars * 8 + 16;
   static_assert(kBars % 8 == 0 && kSmem <= 232448, "shared memory");
-  // TMEM columns
+  // TMEM columns: two buffers of scores (P takes the first half of its own), P V, Q S;
+  // D uses P V's columns, which the carry warps have left by the time P is ready
   static constexpr uint32_t kScores = 0;
-  static constexpr uint32_t kIntra = 128;
+  static constexpr uint32_t kIntra = 256;
+  static constexpr uint32_t kDelta = kIntra;
   static constexpr uint32_t kInter = kIntra + DV;
-  static constexpr uint32_t kDelta = kInter + DV;
 };
 
 template <int DK, int DV, int PARTS>
@@ -253,6 +254,19 @@ __device__ __forceinline__ bool elect_one() {
       "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(p));
   return p != 0;
+}
+
+// Whether phase `parity` of a barrier is complete, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 // Byte offset of 16-byte piece `q` (8 columns) of row r in a 128-byte-swizzled
@@ -440,14 +454,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* full_v = bars + 4;        // [2]
   uint64_t* empty_q = bars + 6;       // [2] scores and Q S read it, outputs left it
   uint64_t* empty_kv = bars + 8;      // [2] a chunk's K and V
-  uint64_t* scores_done = bars + 10;
-  uint64_t* p_ready = bars + 11;
-  uint64_t* out_done = bars + 12;
-  uint64_t* out_read = bars + 13;
-  uint64_t* kw_ready = bars + 14;
-  uint64_t* delta_done = bars + 15;
-  uint64_t* carry_ready = bars + 16;
-  uint64_t* drained = bars + 17;
+  uint64_t* scores_done = bars + 10;  // [2]
+  uint64_t* p_ready = bars + 12;      // [2] the score warps may be a chunk ahead
+  uint64_t* out_done = bars + 14;
+  uint64_t* out_read = bars + 15;
+  uint64_t* kw_ready = bars + 16;
+  uint64_t* delta_done = bars + 17;
+  uint64_t* carry_ready = bars + 18;
+  uint64_t* drained = bars + 19;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kNumBars);
 
   const mb_decay_attention_args& a = args.a;
@@ -464,9 +478,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&full_v[s], 1);
       mbar_init(&empty_q[s], 8);
       mbar_init(&empty_kv[s], 1);
+      mbar_init(&scores_done[s], 1);
+      mbar_init(&p_ready[s], 8);
     }
-    mbar_init(scores_done, 1);
-    mbar_init(p_ready, 8);
     mbar_init(out_done, 2);  // the products' completion, and what their operands' makers wrote
     mbar_init(out_read, 8);
     mbar_init(kw_ready, 8);
@@ -543,8 +557,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint64_t ds = mn_desc(smem_addr(smem + L::kS), DK * 128);
       uint32_t it = 0, hand = 0, cin = 0;
       bool ok = true;
-      auto scores = [&](uint32_t j) {
+      // the scores of chunk j, if its Q and K are there (or after waiting for them);
+      // what their buffer held has been read by then
+      uint32_t scored = 0;
+      auto scores = [&](uint32_t j, bool wait) {
         const int s = j & 1;
+        if (!wait && !(mbar_test(&full_q[s], (j >> 1) & 1) && mbar_test(&full_k[s], (j >> 1) & 1))) {
+          return true;
+        }
         if (!mbar_wait_bounded(&full_q[s], (j >> 1) & 1) ||
             !mbar_wait_bounded(&full_k[s], (j >> 1) & 1)) {
           return false;
@@ -553,9 +573,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int k = 0; k < DK / 16; ++k) {
           const uint32_t at = (s * L::kQBytes + (k >> 2) * kBlockBytes + (k & 3) * 32) >> 4;
-          mma_f16(tmem + L::kScores, dq + at, dk + at, i_scores, k != 0);
+          mma_f16(tmem + L::kScores + s * 128, dq + at, dk + at, i_scores, k != 0);
         }
-        mma_commit(scores_done);
+        mma_commit(&scores_done[s]);
+        ++scored;
         return true;
       };
       // the next chunk's scores are issued a chunk ahead, across units
@@ -566,7 +587,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         return x;
       };
       unit = next_unit(unit);
-      if (unit < args.units) ok = scores(0);
+      if (unit < args.units) ok = scores(0, true);
       while (unit < args.units && ok) {
         const Unit u = decode_unit(args, unit);
         const int64_t following = next_unit(unit + gridDim.x);
@@ -575,11 +596,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const uint64_t v0 = dv + (((it % VS) * L::kVBytes) >> 4);
           const bool last = i + 1 == u.chunks;
           ok = false;
-          // what the output accumulators held has been read
+          const bool more = !last || following < args.units;
+          // what the last chunk left in the accumulators and in P has been read
           if (it >= 1 && !mbar_wait_bounded(out_read, (it - 1) & 1)) break;
+          if (more && !scores(it + 1, false)) break;
           if (i > 0 || carry_in) {
-            if (!mbar_wait_bounded(carry_ready, cin & 1)) break;
-            ++cin;
+            // (later chunks' carries were waited for ahead of the last P V)
+            if (i == 0) {
+              if (!mbar_wait_bounded(carry_ready, cin & 1)) break;
+              ++cin;
+            }
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < DK / 16; ++k) {
@@ -602,22 +628,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               mma_f16(tmem + L::kDelta, k0 + k * 128, v0 + k * 128, i_delta, 1u);
             }
             mma_commit(delta_done);
+            if (scored == it + 1 && !scores(it + 1, false)) break;
+            // D has been read: its columns take P V
+            if (!mbar_wait_bounded(carry_ready, cin & 1)) break;
+            ++cin;
           }
-          if (!mbar_wait_bounded(p_ready, it & 1)) break;
+          if (!mbar_wait_bounded(&p_ready[s], (it >> 1) & 1)) break;
           if (!mbar_wait_bounded(&full_v[it % VS], (it / VS) & 1)) break;
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < kC / 16; ++k) {
-            mma_f16_ts(tmem + L::kIntra, tmem + L::kScores + k * 8, v0 + k * 128, i_out, k != 0);
+            mma_f16_ts(tmem + L::kIntra, tmem + L::kScores + s * 128 + k * 8, v0 + k * 128, i_out,
+                       k != 0);
           }
           mma_commit(out_done);
           mma_commit(&empty_kv[s]);
           mbar_arrive(out_done);
-          if (!last || following < args.units) {
-            // the next scores overwrite P: its product has to be complete
-            if (!mbar_wait_bounded(out_done, it & 1)) break;
-            if (!scores(it + 1)) break;
-          }
+          if (more && scored == it + 1 && !scores(it + 1, true)) break;
           ok = true;
         }
         unit = following;
@@ -630,7 +657,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     reg_dec<80>();
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const int r = quarter * 32 + lane;
-    const uint32_t t_scores = tmem + L::kScores + (uint32_t(quarter * 32) << 16);
     const float intra = a.out_scale * a.kv_scale;
     uint32_t it = 0;
     bool ok = true;
@@ -639,13 +665,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int i = 0; i < u.chunks; ++i, ++it) {
         const int s = it & 1;
         const int n = chunk_steps(u, chunk_t0(u, i, reverse));
+        const uint32_t t_scores = tmem + L::kScores + s * 128 + (uint32_t(quarter * 32) << 16);
         ok = false;
+        if (!mbar_wait_bounded(&scores_done[s], (it >> 1) & 1)) break;
         if (n < kC) {
+          // (with one V stage these warps may be here before the last chunk left it)
+          if (VS == 1 && it >= 1 && !mbar_wait_bounded(out_done, (it - 1) & 1)) break;
           if (!mbar_wait_bounded(&full_v[it % VS], (it / VS) & 1)) break;
           if (r >= n) zero_v_row<DV>(smem + L::kV + (it % VS) * L::kVBytes, r, half);
           fence_proxy_async_smem();
         }
-        if (!mbar_wait_bounded(scores_done, it & 1)) break;
         tc_fence_after();
         // column blocks half and half + 2; those wholly on the other side of the
         // diagonal are zero
@@ -714,7 +743,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         tmem_wait_st();
         tc_fence_before();
-        warp_arrive(p_ready, lane);
+        warp_arrive(&p_ready[s], lane);
         ok = true;
       }
     }
@@ -804,7 +833,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           // K <- W_kv K once the scores that read K are complete, and what rounding
           // leaves of it (the last chunk's remainders are used: its D was waited for)
           if (!mbar_wait_bounded(&full_k[s], (it >> 1) & 1)) break;
-          if (!mbar_wait_bounded(scores_done, it & 1)) break;
+          if (!mbar_wait_bounded(&scores_done[s], (it >> 1) & 1)) break;
           if (n < kC) {  // V as the score warps leave it
             if (!mbar_wait_bounded(&full_v[it % VS], (it / VS) & 1)) break;
             if (r >= n) zero_v_row<DV>(smem + L::kV + (it % VS) * L::kVBytes, r, half);
