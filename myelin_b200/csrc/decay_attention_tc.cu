@@ -14,8 +14,8 @@
 //   warp 0      copies: Q, K, V, two stages of 128-byte-swizzled tiles
 //   warp 1      issues the products, one thread: the next chunk's Q K^T, then this one's
 //               Q S, (W_kv K)^T V and P V
-//   warps 4-11  K -> W_kv K in place, then scores -> P (16 bits, back into TMEM as an
-//               A operand); two warps per 32 rows, half of the columns each
+//   warps 4-11  scores -> P (16 bits, back into TMEM as an A operand) and K -> W_kv K
+//               in place; two warps per 32 rows, half of the columns each
 //   warps 12-19 outputs; the carry in fp32 registers (row per lane, half of the
 //               columns), rounded into shared memory as the next chunk's operand
 // Registers move from the first three warpgroups to the last two (setmaxnreg).
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const int r = quarter * 32 + lane;
     const float intra = a.out_scale * a.kv_scale;
-    uint32_t it = 0;
+    uint32_t it = 0, hand = 0;
     bool ok = true;
     for (int64_t unit = blockIdx.x; unit < args.units && ok; unit += gridDim.x) {
       const Unit u = decode_unit(args, unit);
@@ -667,6 +667,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int n = chunk_steps(u, chunk_t0(u, i, reverse));
         const uint32_t t_scores = tmem + L::kScores + s * 128 + (uint32_t(quarter * 32) << 16);
         ok = false;
+        if (!mbar_wait_bounded(&full_k[s], (it >> 1) & 1)) break;
         if (!mbar_wait_bounded(&scores_done[s], (it >> 1) & 1)) break;
         if (n < kC) {
           // (with one V stage these warps may be here before the last chunk left it)
@@ -744,6 +745,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_wait_st();
         tc_fence_before();
         warp_arrive(&p_ready[s], lane);
+        if (i + 1 < u.chunks) {
+          // K <- W_kv K (the scores that read K are complete), and what rounding leaves
+          // of it, once the last chunk's remainders are used
+          if (hand >= 1 && !mbar_wait_bounded(delta_done, (hand - 1) & 1)) break;
+          ++hand;
+          weigh_k_row<T, DK, 2>(smem + L::kK + s * L::kQBytes, smem + L::kLo, r, half,
+                                r < n ? kv_weight(u, r, n, reverse) : 0.0f, r < n);
+          fence_proxy_async_smem();
+          warp_arrive(kw_ready, lane);
+        }
         ok = true;
       }
     }
@@ -830,18 +841,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           owed = false;
         };
         if (i + 1 < u.chunks) {
-          // K <- W_kv K once the scores that read K are complete, and what rounding
-          // leaves of it (the last chunk's remainders are used: its D was waited for)
-          if (!mbar_wait_bounded(&full_k[s], (it >> 1) & 1)) break;
-          if (!mbar_wait_bounded(&scores_done[s], (it >> 1) & 1)) break;
-          if (n < kC) {  // V as the score warps leave it
-            if (!mbar_wait_bounded(&full_v[it % VS], (it / VS) & 1)) break;
-            if (r >= n) zero_v_row<DV>(smem + L::kV + (it % VS) * L::kVBytes, r, half);
-          }
-          weigh_k_row<T, DK, 2>(smem + L::kK + s * L::kQBytes, smem + L::kLo, r, half,
-                                r < n ? kv_weight(u, r, n, reverse) : 0.0f, r < n);
-          fence_proxy_async_smem();
-          warp_arrive(kw_ready, lane);
           release();
           if (!mbar_wait_bounded(delta_done, hand & 1)) break;
           ++hand;
