@@ -327,4 +327,5 @@ class DropoutFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx: Any, g):
         (seed,) = ctx.saved_tensors
-        return DropoutFunction.apply(g, seed, *ctx.cfg), None, None, None
+        again = DropoutFunction.apply if torch.is_grad_enabled() else cops.dropout
+        return again(g, seed, *ctx.cfg), None, None, None

@@ -348,15 +348,16 @@ int check_args(const mb_decay_attention_args* a, const char* what) {
   return 0;
 }
 
-// Segments of the recurrent kernel: enough blocks for every SM (four resident
-// each) when batch x heads x column tiles are few, at least 64 steps apiece (a
-// segment costs a read and a write of its memory, and its keys and values are
-// read twice).
+// Segments of the recurrent kernel: enough blocks for every SM (four resident each)
+// when batch x heads x column tiles are few, at least 128 steps apiece. A split costs
+// a second pass over k and v and two more launches: below four segments, or 1024
+// steps, one pass is as fast (T = 333, 70 blocks: 27 us in one pass, 36 us in five
+// segments).
 AttnSplit recurrent_split(const mb_decay_attention_args& a) {
   const int64_t blocks = a.B * a.H * ceil_div(a.Dv, kCols);
   int64_t segments = blocks > 0 ? (148 * 4) / blocks : 1;
-  segments = imin64(segments, a.T / 64);
-  if (segments < 4) segments = 1;  // the extra pass over k and v costs more than it gains
+  segments = imin64(segments, a.T / 128);
+  if (segments < 4 || a.T < 1024) segments = 1;
   const int64_t len = segments > 1 ? ceil_div(a.T, segments) : a.T;
   segments = segments > 1 ? ceil_div(a.T, len) : 1;
   return AttnSplit{static_cast<int>(segments), len, nullptr};

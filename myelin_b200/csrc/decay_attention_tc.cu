@@ -51,6 +51,7 @@ struct TcArgs {
   int64_t units;  // segments x B x H
   // whether a dimension's coordinate counts (0: the tensor is broadcast along it)
   int32_t q_b, q_h, k_b, k_h, v_b, v_h, o_b, o_h;
+  int32_t m_map;  // states: memories leave by tensor stores
 };
 
 template <int DK, int DV>
@@ -90,7 +91,8 @@ struct StatesLayout {
   static constexpr int kK = 0;  // two stages each
   static constexpr int kLo = kK + 2 * kKBytes;  // the further parts of W_kv K
   static constexpr int kV = kLo + (PARTS - 1) * kKBytes;
-  static constexpr int kBars = kV + 2 * kVBytes;
+  static constexpr int kOut = kV + 2 * kVBytes;  // 32 x 32 fp32 per carry warp, on the way out
+  static constexpr int kBars = kOut + 8 * 4096;
   static constexpr int kNumBars = 12;
   static constexpr size_t kSmem = kBars + kNumBars * 8 + 16;
   static_assert(kSmem <= 232448, "shared memory");
@@ -946,6 +948,7 @@ template <typename T, int DK, int DV>
 __global__ void __launch_bounds__(kTcThreads, 1)
     attn_states_kernel(const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v,
+                       const __grid_constant__ CUtensorMap map_m,
                        const __grid_constant__ TcArgs args) {
   constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
   using L = StatesLayout<DK, DV, PARTS>;
@@ -1134,8 +1137,33 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         warp_arrive(delta_read, lane);
         ok = true;
       }
-      if (ok) store_memory_row<kCols>(to, to_sc, a.Dv - col0, S);
+      if (!ok) break;
+      if (args.m_map) {
+        // whole 128-byte rows by tensor stores, 32 x 32 values at a time (a lane's own
+        // row-wise stores touch 32 lines per instruction)
+        if (holds) {
+          uint8_t* block = smem + L::kOut + (warp - 12) * 4096;
+#pragma unroll
+          for (int c0 = 0; c0 < kCols; c0 += 32) {
+            if (lane == 0) tma_store_wait_read<0>();
+            __syncwarp();
+            float x[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = S[c0 + j];
+            stage_row32<float>(block, lane, 0, x);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && quarter * 32 < a.Dk && col0 + c0 < a.Dv) {
+              const int z = static_cast<int>(whole ? u.b : u.seg * a.B + u.b);
+              tma_store_4d(&map_m, block, col0 + c0, quarter * 32, u.h, z);
+            }
+          }
+        }
+      } else {
+        store_memory_row<kCols>(to, to_sc, a.Dv - col0, S);
+      }
     }
+    if (lane == 0) tma_store_wait_all();
   }
   tmem_free(tmem, warp);
 }
@@ -1162,6 +1190,38 @@ bool make_attn_map(CUtensorMap* map, const mb_steps& x, int64_t T, int64_t H, in
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A [col, row, h, b] map of 32 x 32 boxes over the memories that the states kernel
+// writes: `last`, or with several segments the workspace (its segments and rows as
+// one dimension). False where their rows are not whole 16-byte pieces.
+bool make_memory_map(CUtensorMap* map, const mb_decay_attention_args& a, const AttnSplit& split) {
+  auto fn = tma_encode_fn();
+  mb_memory m = a.last;
+  int64_t outer = a.B;
+  if (split.segments > 1) {
+    m.data = split.states;
+    m.stride_col = 1;
+    m.stride_row = a.Dv;
+    m.stride_h = a.Dk * a.Dv;
+    m.stride_b = a.H * m.stride_h;
+    outer = split.segments * a.B;
+  }
+  if (fn == nullptr || m.stride_col != 1 || !aligned_to(m.data, 16)) return false;
+  const int64_t strides64[3] = {m.stride_row, a.H > 1 ? m.stride_h : 4, outer > 1 ? m.stride_b : 4};
+  for (int64_t x : strides64) {
+    if (x <= 0 || x % 4 != 0 || x >= (int64_t(1) << 37)) return false;
+  }
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.Dv), static_cast<cuuint64_t>(a.Dk),
+                        static_cast<cuuint64_t>(a.H), static_cast<cuuint64_t>(outer)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(strides64[0] * 4),
+                           static_cast<cuuint64_t>(strides64[1] * 4),
+                           static_cast<cuuint64_t>(strides64[2] * 4)};
+  cuuint32_t box[4] = {32, 32, 1, 1};
+  cuuint32_t estride[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, m.data, dims, strides, box, estride,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int attn_sm_count() {
   int dev = 0, n = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) {
@@ -1172,14 +1232,17 @@ int attn_sm_count() {
 
 template <typename T, int DK, int DV>
 int launch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-              const CUtensorMap& mo, const TcArgs& args, bool states, cudaStream_t s) {
+              const CUtensorMap& mo, TcArgs args, bool states, cudaStream_t s) {
   const unsigned grid = static_cast<unsigned>(imin64(args.units, attn_sm_count()));
   if (states) {
     constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
     constexpr size_t smem = StatesLayout<DK, DV, PARTS>::kSmem;
     auto kern = attn_states_kernel<T, DK, DV>;
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    kern<<<grid, kTcThreads, smem, s>>>(mk, mv, args);
+    CUtensorMap mm;
+    memset(&mm, 0, sizeof(mm));
+    args.m_map = make_memory_map(&mm, args.a, args.split) ? 1 : 0;
+    kern<<<grid, kTcThreads, smem, s>>>(mk, mv, mm, args);
     MB_CHECK_LAUNCH("mb_decay_attention (states)");
   } else {
     constexpr size_t smem = OutLayout<DK, DV>::kSmem;
@@ -1199,6 +1262,7 @@ int launch_type(const mb_decay_attention_args& a, const AttnSplit& split, bool s
   args.a = a;
   args.split = split;
   args.units = split.segments * a.B * a.H;
+  args.m_map = 0;
   const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   CUtensorMap mq, mk, mv, mo;
   MB_CHECK_ARG(make_attn_map(&mq, a.q, a.T, a.H, a.B, a.Dk, bf16, kC, &args.q_h, &args.q_b) &&
