@@ -44,6 +44,7 @@ from myelin_b200.kernels import (
 )
 from myelin_b200.modules import (
     ALIFCell,
+    DecayAttention,
     IzhikevichCell,
     LIFCell,
     LinearLIF,

@@ -7,16 +7,17 @@
 namespace mb {
 namespace {
 
-constexpr int kCols = 32;       // memory columns (of Dv) per block: one per lane
 constexpr int kRecThreads = 256;
 constexpr int kRecWarps = kRecThreads / 32;
 
-__host__ __device__ constexpr int rec_steps(int rows) { return rows >= 32 ? 8 : 16; }
+__host__ __device__ constexpr int rec_steps(int rows, int cols) {
+  return rows >= 32 || cols > 1 ? 8 : 16;
+}
 
 // ---------------------------------------------------------------------------
 // Recurrent kernel: any head size up to 256, any element type and stride, sums in
-// fp32. A block holds 32 columns of one memory in registers (lane = column, each
-// warp R of the Dk rows), stages TC steps of q, k and v in shared memory as fp32
+// fp32. A block holds 32 C columns of one memory in registers (C per lane, each warp
+// R of the Dk rows), stages TC steps of q, k and v in shared memory as fp32
 // (the next ones on their way meanwhile), walks them without a barrier and then adds
 // the eight warps' partial outputs.
 //
@@ -27,7 +28,10 @@ __host__ __device__ constexpr int rec_steps(int rows) { return rows >= 32 ? 8 : 
 // with the leak of the first step applied before a forward burst, that of the last
 // one after a reverse burst. The powers are formed in double, so that g^-p g^p is 1
 // to two roundings. Decays below 0.02 (whose powers would leave fp32's range) take
-// bursts of one step. About 2 Dk Dv FMAs per step and head bound it.
+// bursts of one step. About 2 Dk Dv FMAs per step and head bound it, once a lane has
+// several columns: a broadcast 16-byte read of k or q fills a warp's registers in four
+// cycles whatever it is used for, so that with one column per lane those reads took
+// 0.906 ms at T=1024, 256 rows of 128 x 128 heads (19 TFLOP/s).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
   uint64_t r;
@@ -38,11 +42,12 @@ __device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
   return *reinterpret_cast<float2*>(&r);
 }
 
-template <typename T, int R, bool STATES_ONLY>
+template <typename T, int R, int C, bool STATES_ONLY>
 __global__ void __launch_bounds__(kRecThreads)
     attn_recurrent_kernel(const __grid_constant__ mb_decay_attention_args a,
                           const __grid_constant__ AttnSplit split) {
-  constexpr int TC = rec_steps(R);
+  constexpr int TC = rec_steps(R, C);
+  constexpr int kCols = 32 * C;
   constexpr int ROWS = R * kRecWarps;
   constexpr int NK = TC * ROWS / kRecThreads;               // staged k (q) elements per thread
   constexpr int NV = (TC * kCols + kRecThreads - 1) / kRecThreads;
@@ -61,8 +66,7 @@ __global__ void __launch_bounds__(kRecThreads)
   u /= a.H;
   const int64_t b = u % a.B;
   const int64_t seg = u / a.B;
-  const int64_t col0 = tile * kCols, col = col0 + lane;
-  const bool col_ok = col < a.Dv;
+  const int64_t col0 = tile * kCols;
   const int row0 = warp * R;
 
   const int64_t L = attn_row_length(a.lengths, b, a.T);
@@ -85,21 +89,25 @@ __global__ void __launch_bounds__(kRecThreads)
     if (threadIdx.x < TC) s_inv[threadIdx.x] = burst == 1 ? 1.0f : static_cast<float>(1.0 / p);
   }
 
-  float2 S[R / 2];
+  float2 S[C][R / 2];  // columns col0 + lane + 32 c
   const int64_t seg_at = ((seg * a.B + b) * a.H + h) * a.Dk;
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int64_t r = row0 + i;
-    float x = 0.0f;
-    if (col_ok && r < a.Dk && !STATES_ONLY) {
-      if (split.segments > 1) {
-        x = split.states[(seg_at + r) * a.Dv + col];
-      } else if (a.first.data != nullptr) {
-        x = a.first.data[b * a.first.stride_b + h * a.first.stride_h + r * a.first.stride_row +
-                         col * a.first.stride_col];
+  for (int c = 0; c < C; ++c) {
+    const int64_t col = col0 + lane + 32 * c;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t r = row0 + i;
+      float x = 0.0f;
+      if (col < a.Dv && r < a.Dk && !STATES_ONLY) {
+        if (split.segments > 1) {
+          x = split.states[(seg_at + r) * a.Dv + col];
+        } else if (a.first.data != nullptr) {
+          x = a.first.data[b * a.first.stride_b + h * a.first.stride_h + r * a.first.stride_row +
+                           col * a.first.stride_col];
+        }
       }
+      (i & 1 ? S[c][i / 2].y : S[c][i / 2].x) = x;
     }
-    (i & 1 ? S[i / 2].y : S[i / 2].x) = x;
   }
 
   // this thread's elements of the next steps' k, q and v
@@ -126,7 +134,10 @@ __global__ void __launch_bounds__(kRecThreads)
   auto scale_memory = [&](float w) {
     const float2 w2 = make_float2(w, w), zero = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < R / 2; ++i) S[i] = fma_pair(S[i], w2, zero);
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int i = 0; i < R / 2; ++i) S[c][i] = fma_pair(S[c][i], w2, zero);
+    }
   };
   if (n > 0) fetch(0);
   for (int64_t p0 = 0; p0 < n; p0 += TC) {
@@ -148,22 +159,41 @@ __global__ void __launch_bounds__(kRecThreads)
     for (int s0 = 0; s0 < steps; s0 += burst) {
       const int s1 = min(steps, s0 + burst);
       if (!reverse) scale_memory(g);
-#pragma unroll 2
-      for (int s = s0; s < s1; ++s) {
-        const float2 vc = make_float2(sv[s][lane], sv[s][lane]);
-        float2 acc = make_float2(0.0f, 0.0f), acc2 = make_float2(0.0f, 0.0f);
+      auto step = [&](int s) {
+        float2 vc[C], acc[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const float x = sv[s][lane + 32 * c];
+          vc[c] = make_float2(x, x);
+          acc[c] = make_float2(0.0f, 0.0f);
+        }
 #pragma unroll
         for (int i = 0; i < R; i += 4) {
           const float4 kk = *reinterpret_cast<const float4*>(&sk[s][row0 + i]);
-          S[i / 2] = fma_pair(make_float2(kk.x, kk.y), vc, S[i / 2]);
-          S[i / 2 + 1] = fma_pair(make_float2(kk.z, kk.w), vc, S[i / 2 + 1]);
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            S[c][i / 2] = fma_pair(make_float2(kk.x, kk.y), vc[c], S[c][i / 2]);
+            S[c][i / 2 + 1] = fma_pair(make_float2(kk.z, kk.w), vc[c], S[c][i / 2 + 1]);
+          }
           if constexpr (!STATES_ONLY) {
             const float4 qq = *reinterpret_cast<const float4*>(&sq[s][row0 + i]);
-            acc = fma_pair(make_float2(qq.x, qq.y), S[i / 2], acc);
-            acc2 = fma_pair(make_float2(qq.z, qq.w), S[i / 2 + 1], acc2);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              acc[c] = fma_pair(make_float2(qq.x, qq.y), S[c][i / 2], acc[c]);
+              acc[c] = fma_pair(make_float2(qq.z, qq.w), S[c][i / 2 + 1], acc[c]);
+            }
           }
         }
-        if constexpr (!STATES_ONLY) part[s][warp][lane] = (acc.x + acc.y) + (acc2.x + acc2.y);
+        if constexpr (!STATES_ONLY) {
+#pragma unroll
+          for (int c = 0; c < C; ++c) part[s][warp][lane + 32 * c] = acc[c].x + acc[c].y;
+        }
+      };
+      if (s1 - s0 == TC) {  // whole bursts unrolled: the steps' loads run ahead of their sums
+#pragma unroll
+        for (int s = 0; s < TC; ++s) step(s);
+      } else {
+        for (int s = s0; s < s1; ++s) step(s);
       }
       scale_memory(s_pow[reverse ? s1 - s0 : s1 - s0 - 1]);
     }
@@ -188,18 +218,22 @@ __global__ void __launch_bounds__(kRecThreads)
       if (c < a.Dv) o[t * a.o.stride_t + c] = Elem<T>::zero();
     }
   }
-  if (!col_ok) return;
   const bool whole = !STATES_ONLY && split.segments == 1 && a.last.data != nullptr;
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int64_t r = row0 + i;
-    const float x = i & 1 ? S[i / 2].y : S[i / 2].x;
-    if (r >= a.Dk) continue;
-    if constexpr (STATES_ONLY) {
-      split.states[(seg_at + r) * a.Dv + col] = x;
-    } else if (whole) {
-      a.last.data[b * a.last.stride_b + h * a.last.stride_h + r * a.last.stride_row +
-                  col * a.last.stride_col] = x;
+  for (int c = 0; c < C; ++c) {
+    const int64_t col = col0 + lane + 32 * c;
+    if (col >= a.Dv) continue;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t r = row0 + i;
+      const float x = i & 1 ? S[c][i / 2].y : S[c][i / 2].x;
+      if (r >= a.Dk) continue;
+      if constexpr (STATES_ONLY) {
+        split.states[(seg_at + r) * a.Dv + col] = x;
+      } else if (whole) {
+        a.last.data[b * a.last.stride_b + h * a.last.stride_h + r * a.last.stride_row +
+                    col * a.last.stride_col] = x;
+      }
     }
   }
 }
@@ -348,14 +382,22 @@ int check_args(const mb_decay_attention_args* a, const char* what) {
   return 0;
 }
 
-// Segments of the recurrent kernel: enough blocks for every SM (four resident each)
+// Columns per lane: as many as the head has (four only while a warp's rows fit its
+// registers), fewer where that leaves less than two blocks per SM.
+int recurrent_cols(const mb_decay_attention_args& a) {
+  int c = a.Dv > 64 && a.Dk <= 128 ? 4 : a.Dv > 32 ? 2 : 1;
+  const int64_t most = a.T >= 1024 ? a.T / 128 : 1;  // segments
+  while (c > 1 && a.B * a.H * ceil_div(a.Dv, 32 * c) * most < 2 * 148) c /= 2;
+  return c;
+}
+
+// Segments of the recurrent kernel: enough blocks for every SM (two resident each)
 // when batch x heads x column tiles are few, at least 128 steps apiece. A split costs
 // a second pass over k and v and two more launches: below four segments, or 1024
-// steps, one pass is as fast (T = 333, 70 blocks: 27 us in one pass, 36 us in five
-// segments).
+// steps, one pass is as fast.
 AttnSplit recurrent_split(const mb_decay_attention_args& a) {
-  const int64_t blocks = a.B * a.H * ceil_div(a.Dv, kCols);
-  int64_t segments = blocks > 0 ? (148 * 4) / blocks : 1;
+  const int64_t blocks = a.B * a.H * ceil_div(a.Dv, 32 * recurrent_cols(a));
+  int64_t segments = blocks > 0 ? (148 * 2) / blocks : 1;
   segments = imin64(segments, a.T / 128);
   if (segments < 4 || a.T < 1024) segments = 1;
   const int64_t len = segments > 1 ? ceil_div(a.T, segments) : a.T;
@@ -363,20 +405,31 @@ AttnSplit recurrent_split(const mb_decay_attention_args& a) {
   return AttnSplit{static_cast<int>(segments), len, nullptr};
 }
 
-template <typename T, int R>
-int launch_recurrent_r(const mb_decay_attention_args& a, const AttnSplit& split, bool states_only,
-                       cudaStream_t stream) {
-  const int64_t blocks = split.segments * a.B * a.H * ceil_div(a.Dv, kCols);
+template <typename T, int R, int C>
+int launch_recurrent_rc(const mb_decay_attention_args& a, const AttnSplit& split, bool states_only,
+                        cudaStream_t stream) {
+  const int64_t blocks = split.segments * a.B * a.H * ceil_div(a.Dv, 32 * C);
   MB_CHECK_ARG(blocks <= 0x7fffffff, "mb_decay_attention: too many (batch, head) rows");
   if (states_only) {
-    attn_recurrent_kernel<T, R, true>
+    attn_recurrent_kernel<T, R, C, true>
         <<<static_cast<unsigned>(blocks), kRecThreads, 0, stream>>>(a, split);
   } else {
-    attn_recurrent_kernel<T, R, false>
+    attn_recurrent_kernel<T, R, C, false>
         <<<static_cast<unsigned>(blocks), kRecThreads, 0, stream>>>(a, split);
   }
   MB_CHECK_LAUNCH("mb_decay_attention");
   return 0;
+}
+
+template <typename T, int R>
+int launch_recurrent_r(const mb_decay_attention_args& a, const AttnSplit& split, bool states_only,
+                       cudaStream_t stream) {
+  const int c = recurrent_cols(a);
+  if constexpr (R <= 16) {
+    if (c == 4) return launch_recurrent_rc<T, R, 4>(a, split, states_only, stream);
+  }
+  if (c >= 2) return launch_recurrent_rc<T, R, 2>(a, split, states_only, stream);
+  return launch_recurrent_rc<T, R, 1>(a, split, states_only, stream);
 }
 
 template <typename T>

@@ -10,11 +10,17 @@ length one.
 
 from __future__ import annotations
 
+import math
 from typing import Literal
 
 import torch
 from torch import nn
 
+from myelin_b200.attention import (
+    DecayAttentionState,
+    decay_attention_forward,
+    decay_attention_step,
+)
 from myelin_b200.checkpointing import CheckpointSize
 from myelin_b200.dropout import spike_dropout
 from myelin_b200.kernels import (
@@ -390,6 +396,87 @@ class SpikeDropout(nn.Module):
         return f"p={self.p}, time_shared={self.time_shared}"
 
 
+class DecayAttention(nn.Module):
+    """A layer of leaky associative memories: projections to queries, keys and values,
+    attention with a decay for each head, dropout and an output projection.
+
+    Each head's memory leaks with its own time constant, spaced evenly in the
+    logarithm from ``tau_min`` to ``tau_max`` steps (decay ``1 - 1 / tau``, as
+    ``LIFParams.decay``). ``forward`` takes ``[T, B, in_features]`` and carries the
+    memories from ``initial_state`` to the state it returns; ``step`` takes one
+    time step ``[B, in_features]``. Dropout (``SpikeDropout``, one mask for all
+    steps) applies in training mode, in ``forward`` only.
+    """
+
+    def __init__(
+        self,
+        in_features: int,
+        heads: int,
+        key_size: int,
+        value_size: int | None = None,
+        out_features: int | None = None,
+        *,
+        tau_min: float = 4.0,
+        tau_max: float = 512.0,
+        dropout: float = 0.0,
+        bias: bool = True,
+    ) -> None:
+        super().__init__()
+        if heads < 1 or key_size < 1:
+            raise ValueError("heads and key_size must be at least 1")
+        if not 1.0 <= tau_min <= tau_max:
+            raise ValueError("tau_min must be at least 1 and tau_max at least tau_min")
+        self.heads, self.key_size = heads, key_size
+        self.value_size = key_size if value_size is None else value_size
+        width = heads * self.value_size
+        self.queries = LinearSynapse(in_features, heads * key_size, bias=bias)
+        self.keys = LinearSynapse(in_features, heads * key_size, bias=bias)
+        self.values = LinearSynapse(in_features, width, bias=bias)
+        self.output = LinearSynapse(width, in_features if out_features is None else out_features,
+                                    bias=bias)
+        self.dropout = SpikeDropout(dropout)
+        tau = torch.logspace(math.log2(tau_min), math.log2(tau_max), heads, base=2.0,
+                             dtype=torch.float64)
+        self.register_buffer("decay", (1.0 - 1.0 / tau).float())
+
+    def _apply(self, fn, recurse=True):
+        # a change of dtype is for the projections; decays stay fp32
+        decay = self.decay
+        super()._apply(fn, recurse)
+        self.decay = decay.to(self.decay.device)
+        return self
+
+    def _heads(self, inputs: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        lead = inputs.shape[:-1]
+        return (self.queries(inputs).view(*lead, self.heads, self.key_size),
+                self.keys(inputs).view(*lead, self.heads, self.key_size),
+                self.values(inputs).view(*lead, self.heads, self.value_size))
+
+    def forward(
+        self,
+        inputs: torch.Tensor,
+        initial_state: DecayAttentionState | None = None,
+        lengths: torch.Tensor | None = None,
+    ) -> tuple[DecayAttentionState, torch.Tensor]:
+        q, k, v = self._heads(inputs)
+        state, out = decay_attention_forward(q, k, v, self.decay, initial_state,
+                                             scale=self.key_size**-0.5, lengths=lengths)
+        return state, self.output(self.dropout(out.flatten(-2)))
+
+    def step(
+        self,
+        inputs: torch.Tensor,
+        state: DecayAttentionState,
+        active: torch.Tensor | None = None,
+        *,
+        inplace: bool = False,
+    ) -> tuple[DecayAttentionState, torch.Tensor]:
+        q, k, v = self._heads(inputs)
+        state, out = decay_attention_step(q, k, v, self.decay, state, scale=self.key_size**-0.5,
+                                          active=active, inplace=inplace)
+        return state, self.output(out.flatten(-2))
+
+
 class RateReadoutClassifier(nn.Module):
     """Hidden streamed LIF layer plus a rate readout (src/myelin/modules.py:848-903).
 
@@ -482,12 +569,14 @@ class LinearSurrogateLIFPacked(nn.Module):
 
 
 def quantize_synapses(module: nn.Module) -> nn.Module:
-    """Replace the synapses of every ``LinearLIF`` and ``LinearSurrogateLIF`` in
-    ``module`` (itself included) by 8-bit ones, in place, for inference; returns
-    ``module``. Rate readouts and packed layers keep theirs: their projection is
-    part of a fused function that takes float weights."""
+    """Replace the synapses of every ``LinearLIF``, ``LinearSurrogateLIF`` and
+    ``DecayAttention`` in ``module`` (itself included) by 8-bit ones, in place, for
+    inference; returns ``module``. Rate readouts and packed layers keep theirs:
+    their projection is part of a fused function that takes float weights."""
 
     for m in module.modules():
-        if isinstance(m, LinearLIF | LinearSurrogateLIF) and isinstance(m.synapse, LinearSynapse):
-            m.synapse = QuantizedLinearSynapse.from_synapse(m.synapse)
+        if isinstance(m, LinearLIF | LinearSurrogateLIF | DecayAttention):
+            for name, child in m.named_children():
+                if isinstance(child, LinearSynapse):
+                    setattr(m, name, QuantizedLinearSynapse.from_synapse(child))
     return module
