@@ -457,6 +457,7 @@ int mb_count_columns_noalloc(const int32_t* words, int64_t rows, int64_t n, int6
  * `first` (optional, zeros without it) is S_{-1}, or H past the last step;
  * `last` (optional) receives the final S, or H_0. Outputs at steps past the
  * row's length are zero, and what the inputs hold there is not used.
+ * `last` may not overlap `first`, nor `o` any input.
  * q, k: [T, B, H, Dk], v, o: [T, B, H, Dv] of `dtype`, element strides per step,
  * row and head, contiguous along the head; first, last: fp32 [B, H, Dk, Dv] with
  * four element strides. Head sizes 1..256. The three gradients are calls of the

@@ -510,6 +510,8 @@ extern "C" int mb_decay_attention(const mb_decay_attention_args* args, void* wor
   MB_CHECK_ARG(a.T == 0 || (a.q.data != nullptr && a.k.data != nullptr && a.v.data != nullptr &&
                             a.o.data != nullptr),
                "mb_decay_attention: q, k, v and o must not be null");
+  MB_CHECK_ARG(a.last.data == nullptr || a.last.data != a.first.data,
+               "mb_decay_attention: last must not be the buffer of first");
   if (a.T == 0 && a.last.data == nullptr) return 0;
   const bool tc = attn_tc_supported(a);
   AttnSplit split = choose_split(a, tc);

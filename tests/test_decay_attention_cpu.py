@@ -164,3 +164,6 @@ def test_c_entry_empty_and_workspace():
     one.q.data = one.k.data = one.v.data = one.o.data = 4096
     assert lib.mb_decay_attention(ctypes.addressof(one), None, 0, None) != 0
     assert "workspace" in lib.mb_last_error().decode()
+    one.first.data = one.last.data = 8192  # the outputs read `first` after `last` is written
+    assert lib.mb_decay_attention(ctypes.addressof(one), None, 0, None) != 0
+    assert "must not be the buffer of first" in lib.mb_last_error().decode()

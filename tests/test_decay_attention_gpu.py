@@ -21,6 +21,7 @@ import torch
 
 import myelin_b200 as mb
 from myelin_b200 import _native as nat
+from myelin_b200 import compile_ops as cops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -428,3 +429,111 @@ def test_wait_timeout_is_reported():
     nat.debug_wait_timeout(nat.MB_UNIT_ATTENTION)
     torch.cuda.synchronize()
     assert nat.device_status() == 1 and nat.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_and_heads_do_not_touch_one_another(dtype):
+    """A row's result is the same bits whatever its neighbours hold, NaN included,
+    and however many there are."""
+
+    T, B, H, D = 300, 4, 3, 64
+    q, k, v = (_randn((T, B, H, D), s, dtype) for s in (1, 2, 3))
+    memory = _randn((B, H, D, D), 4)
+    base, out = mb.decay_attention_forward(q, k, v, _decay(H), mb.DecayAttentionState(memory),
+                                           scale=0.1)
+    for x in (q, k, v):
+        x[:, 1, 2] = float("nan")
+        x[:, 3, 0] = float("inf")
+    state, got = mb.decay_attention_forward(q, k, v, _decay(H), mb.DecayAttentionState(memory),
+                                            scale=0.1)
+    keep = torch.ones((B, H), dtype=torch.bool, device=DEV)
+    keep[1, 2] = keep[3, 0] = False
+    assert torch.equal(got[:, keep], out[:, keep])
+    assert torch.equal(state.memory[keep], base.memory[keep])
+    state, got = mb.decay_attention_forward(q[:, :1], k[:, :1], v[:, :1], _decay(H),
+                                            mb.DecayAttentionState(memory[:1]), scale=0.1)
+    assert torch.equal(got, out[:, :1]) and torch.equal(state.memory, base.memory[:1])
+
+
+def test_a_later_value_does_not_reach_earlier_chunks():
+    T, D = 400, 64
+    q, k, v = (_randn((T, 1, 1, D), s, torch.bfloat16) for s in (1, 2, 3))
+    _, out = mb.decay_attention_forward(q, k, v, _decay(1), scale=0.1)
+    k2, v2 = k.clone(), v.clone()
+    k2[300], v2[300] = float("nan"), float("inf")
+    _, got = mb.decay_attention_forward(q, k2, v2, _decay(1), scale=0.1)
+    assert torch.equal(got[:256], out[:256])  # chunks of 128 steps before the one that holds it
+    assert not torch.isfinite(got[300:]).any()
+
+
+def test_opcheck():
+    T, B, H, D = 20, 2, 2, 16
+    q, k, v = (_randn((T, B, H, D), s, torch.bfloat16) for s in (1, 2, 3))
+    m, lengths = _randn((B, H, D, D), 4), torch.tensor([20, 7], dtype=torch.int32, device=DEV)
+    args = (q, k, v, _decay(H), m, lengths, 0.5)
+    torch.library.opcheck(cops.decay_attention_op, args)
+    torch.library.opcheck(cops.decay_attention_backward_op,
+                          (*args[:6], q, m, 0.5, True, False, True, True))
+    step = (q[0], k[0], v[0], _decay(H), m, None, 0.5)
+    torch.library.opcheck(cops.decay_attention_step_op, step)
+    torch.library.opcheck(cops.decay_attention_step_inplace_op, step)
+
+
+def test_compiled_layer_matches_eager():
+    torch.manual_seed(0)
+    layer = mb.DecayAttention(32, 2, 16).to(DEV)
+    x = torch.randn((40, 2, 32), device=DEV)
+    fast = torch.compile(layer, fullgraph=True)
+    state, out = layer(x)
+    state2, out2 = fast(x)
+    assert (out - out2).abs().max() <= 1e-4 * out.abs().max()
+    g1 = torch.autograd.grad(out.sum(), list(layer.parameters()), allow_unused=True)
+    g2 = torch.autograd.grad(out2.sum(), list(layer.parameters()), allow_unused=True)
+    for a, b in zip(g1, g2):
+        assert (a - b).abs().max() <= 1e-4 * a.abs().max()
+
+
+def test_calls_on_two_streams_at_once():
+    """Split time axes with workspaces of their own, both in flight."""
+
+    T, B, H, D = 4096, 1, 2, 64
+    sets = [[_randn((T, B, H, D), s + 10 * i, torch.bfloat16) for s in (1, 2, 3)] for i in (0, 1)]
+    want = [mb.decay_attention_forward(*x, _decay(H), scale=0.1) for x in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(4):
+        for stream, x in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                got.append(mb.decay_attention_forward(*x, _decay(H), scale=0.1))
+    torch.cuda.synchronize()
+    for i, (state, out) in enumerate(got):
+        assert torch.equal(out, want[i % 2][1])
+        assert torch.equal(state.memory, want[i % 2][0].memory)
+
+
+def test_training_step_in_a_graph():
+    T, B, H, D = 150, 2, 2, 64
+    q, k, v = (_randn((T, B, H, D), s, torch.bfloat16) for s in (1, 2, 3))
+    go = _randn((T, B, H, D), 5, torch.bfloat16)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+
+    def step():
+        _, out = mb.decay_attention_forward(*leaves, decay, scale=0.1)
+        return (out, *torch.autograd.grad(out, leaves, go))
+
+    decay = _decay(H)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    with torch.no_grad():
+        leaves[0].copy_(_randn((T, B, H, D), 9, torch.bfloat16))
+    graph.replay()
+    held = [x.detach().clone() for x in held]
+    for a, b in zip(held, step()):
+        assert torch.equal(a, b)

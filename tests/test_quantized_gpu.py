@@ -94,7 +94,7 @@ def test_rows_that_are_not_finite_or_tiny():
 
 
 SIZES = [(1, 1, 1), (1, 33, 16), (2, 5, 100), (3, 70, 1000), (4, 257, 4096), (4, 9, 8192),
-         (5, 64, 128), (17, 1001, 784), (128, 32, 64), (129, 130, 129), (200, 200, 4112),
+         (5, 64, 128), (9, 40, 3), (200, 1, 64), (17, 1001, 784), (128, 32, 64), (129, 130, 129), (200, 200, 4112),
          (300, 1000, 333), (2000, 2304, 640), (2600, 2561, 200)]
 
 
