@@ -240,7 +240,8 @@ __global__ void __launch_bounds__(kRecThreads)
 
 // Between the two launches of a split time axis: every segment's own memory
 // becomes the carry it starts from, in processing order; the last carry is the
-// final memory. One thread per memory element; `segments` reads and writes.
+// final memory. One thread per memory element; `segments` reads and writes (a
+// length past the row's end decays nothing).
 __global__ void __launch_bounds__(256)
     attn_segment_scan_kernel(const __grid_constant__ mb_decay_attention_args a,
                              const __grid_constant__ AttnSplit split) {
@@ -257,14 +258,23 @@ __global__ void __launch_bounds__(256)
     carry = a.first.data[b * a.first.stride_b + h * a.first.stride_h + r * a.first.stride_row +
                          c * a.first.stride_col];
   }
-  for (int i = 0; i < split.segments; ++i) {
-    const int64_t s = a.reverse ? split.segments - 1 - i : i;
-    const int64_t left = L - s * split.len;
-    const int64_t n = left < 0 ? 0 : imin64(left, split.len);
-    float* at = split.states + s * total + e;
-    const float own = *at;
-    *at = carry;
-    carry = fmaf(decay_pow(log2g, n), carry, own);
+  constexpr int FLIGHT = 8;  // segments' memories on their way at once
+  for (int i0 = 0; i0 < split.segments; i0 += FLIGHT) {
+    float own[FLIGHT];
+#pragma unroll
+    for (int x = 0; x < FLIGHT; ++x) {
+      const int s = a.reverse ? split.segments - 1 - i0 - x : i0 + x;
+      if (i0 + x < split.segments) own[x] = split.states[s * total + e];
+    }
+#pragma unroll
+    for (int x = 0; x < FLIGHT; ++x) {
+      if (i0 + x >= split.segments) break;
+      const int s = a.reverse ? split.segments - 1 - i0 - x : i0 + x;
+      const int64_t left = L - s * split.len;
+      const int64_t n = left < 0 ? 0 : imin64(left, split.len);
+      split.states[s * total + e] = carry;
+      carry = fmaf(decay_pow(log2g, n), carry, own[x]);
+    }
   }
   if (a.last.data != nullptr) {
     a.last.data[b * a.last.stride_b + h * a.last.stride_h + r * a.last.stride_row +

@@ -20,11 +20,15 @@
 //               columns), rounded into shared memory as the next chunk's operand
 // Registers move from the first three warpgroups to the last two (setmaxnreg).
 //
-// What bounds it: the bytes of q, k, v and o (one read, one write); a chunk of
-// 128-wide heads is 128 KB, 5.6 thousand cycles of one SM's share of the copy
-// bandwidth. Its four products are about 100 cycles per 128 x 128 x 16 step
-// (shared-memory reads of both operands bound them), 3.2 thousand in all, and the
-// loop scores -> P -> P V -> next scores about 3.7 thousand.
+// Floor: the bytes of q, k, v and o (one read, one write); a chunk of 128-wide heads is
+// 128 KB, 5.6 thousand cycles of one SM's share of the copy bandwidth. Measured (bf16,
+// 134 M elements each of q, k, v, o): outputs 0.240 ms at T = 256 and 0.282 ms at
+// T = 4096, against 0.164 ms at the copy bandwidth. What holds it there is the chain of
+// one chunk's hand-overs (Q S -> D -> carry -> P V -> outputs read -> next Q S, about 7
+// thousand cycles), not a unit: of the cycles, the tensor pipe is active in 18 %, the
+// issue slots in 26 %, DRAM in 36 %. 65 cycles per 128 x 128 x 16 product, 32 (40) of them per
+// chunk, would take 2.1 (2.6) thousand. Memories: 0.15 ms for 134 M elements each of k
+// and v (0.082 at the copy bandwidth, plus the memories' own bytes).
 #include <cuda.h>
 #include <math.h>
 
@@ -401,10 +405,11 @@ __device__ __forceinline__ void store_memory_row(float* p, int64_t stride, int64
 
 // Sixteen scores of one row times c g^distance, zero on the other side of the
 // diagonal: column j of the group lies at distance e0 - j (REVERSE: j - e0) from the
-// row. The weight runs along the columns, one product each; MASKED: the group may
-// touch the diagonal (or, in reverse, column `valid`, where the row's steps end).
-// Selects, not products with zero: what lies outside may be infinite or NaN.
-template <bool REVERSE, bool MASKED>
+// row; in reverse, columns from `valid` on lie past the row's end. The weight runs
+// along the columns, one product each. Selects, not products with zero: what lies
+// outside may be infinite or NaN. (A second copy without the selects, for groups
+// wholly inside, saved instructions but missed the instruction cache: 3 to 7 % slower.)
+template <bool REVERSE>
 __device__ __forceinline__ void weigh16(const uint32_t* v, int e0, int valid, float c,
                                         const Unit& u, float (&f)[16]) {
   const int d = REVERSE ? -1 - e0 : e0 - 16;  // distance one step before the first column
@@ -412,14 +417,9 @@ __device__ __forceinline__ void weigh16(const uint32_t* v, int e0, int valid, fl
 #pragma unroll
   for (int x = 0; x < 16; ++x) {
     const int j = REVERSE ? x : 15 - x;
-    if constexpr (MASKED) {
-      w = j == e0 ? c : w * u.g;
-      const bool in = REVERSE ? j >= e0 && j < valid : j <= e0;
-      f[j] = in ? __uint_as_float(v[j]) * w : 0.0f;
-    } else {
-      w *= u.g;
-      f[j] = __uint_as_float(v[j]) * w;
-    }
+    w = j == e0 ? c : w * u.g;
+    const bool in = REVERSE ? j >= e0 && j < valid : j <= e0;
+    f[j] = in ? __uint_as_float(v[j]) * w : 0.0f;
   }
 }
 
@@ -683,12 +683,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // diagonal are zero
         auto blank = [&](int jb) { return reverse ? jb < quarter : jb > quarter; };
         auto group = [&](const uint32_t* v, int jb, int y, float (&f)[16]) {  // columns jb * 32 + y ..
-          const int e0 = r - jb * 32 - y;
-          if (jb == quarter || (reverse && n < kC)) {
-            weigh16<REVERSE, true>(v + y, e0, n - jb * 32 - y, intra, u, f);
-          } else {
-            weigh16<REVERSE, false>(v + y, e0, 16, intra, u, f);
-          }
+          weigh16<REVERSE>(v + y, r - jb * 32 - y, n - jb * 32 - y, intra, u, f);
         };
         float scale = 1.0f;
         if constexpr (kHalf) {
@@ -878,7 +873,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (kCols == 64) __syncwarp();
           else bar_sync(7 + quarter, 64);
         }
-#pragma unroll
+#pragma unroll 1  // (as code that fits the instruction cache with the other warps')
         for (int c0 = 0; c0 < kCols; c0 += 16) {
           uint32_t x[16], y[16];
           tmem_ld16_issue(tmem + L::kIntra + lanes + col0 + c0, x);
