@@ -722,7 +722,7 @@ def quantize_rows(x2: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return quantize_rows_op(x2) if _tracing() else _quantize_rows_eager(x2)
 
 
-def _i8_operand(t: torch.Tensor) -> torch.Tensor:
+def i8_operand(t: torch.Tensor) -> torch.Tensor:
     """An int8 matrix whose rows the tensor-map copies can read: itself, or a copy."""
 
     if t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1] \
@@ -741,13 +741,13 @@ def _quantized_project_impl(x2: torch.Tensor, x_scale: torch.Tensor | None, weig
         return out
     if x2.dtype == torch.bool:
         x2 = x2.view(torch.int8)
-    weight = _i8_operand(weight)
+    weight = i8_operand(weight)
     if M <= nat.I8_ROWS and M * ((K + 15) // 16 * 16) <= nat.I8_ROWS_BYTES:
         nat.linear_i8_rows(_rows(x2), x_scale, weight, weight_scale, bias, out)
         return out
     if x2.dtype.is_floating_point:
         x2, x_scale = _quantize_rows_eager(x2)
-    nat.gemm_i8(_i8_operand(x2), x_scale, weight, weight_scale, bias, out)
+    nat.gemm_i8(i8_operand(x2), x_scale, weight, weight_scale, bias, out)
     return out
 
 

@@ -22,6 +22,7 @@ from myelin_b200.attention import (
     decay_attention_step,
 )
 from myelin_b200.checkpointing import CheckpointSize
+from myelin_b200.compile_ops import i8_operand
 from myelin_b200.dropout import spike_dropout
 from myelin_b200.kernels import (
     izhikevich_step,
@@ -103,6 +104,7 @@ class QuantizedLinearSynapse(nn.Module):
         scale = self.scale
         super()._apply(fn, recurse)
         self.scale = scale.to(self.scale.device)
+        self.data = i8_operand(self.data)  # a move to another device drops the row pitch
         return self
 
     def forward(self, inputs: torch.Tensor) -> torch.Tensor:

@@ -109,3 +109,12 @@ def test_c_entries():
         assert lib.mb_gemm_i8(*args) != 0 and message in lib.mb_last_error().decode()
     assert lib.mb_linear_i8_rows(0, p, 8, None, p, 16, p, None, 0, 0, p, 4, 5, 4, 8, None) != 0
     assert "at most" in lib.mb_last_error().decode()
+
+
+def test_synapse_keeps_its_row_pitch_across_devices():
+    data = torch.zeros((6, 32), dtype=torch.int8)[:, :20]
+    synapse = mb.QuantizedLinearSynapse(mb.QuantizedWeight(data, torch.ones(6)))
+    synapse.data = data.contiguous()  # as a copy to another device leaves it
+    synapse.half()
+    assert synapse.data.stride(0) % 16 == 0 and synapse.data.shape == (6, 20)
+    assert synapse.scale.dtype == torch.float32
