@@ -537,3 +537,33 @@ def test_training_step_in_a_graph():
     held = [x.detach().clone() for x in held]
     for a, b in zip(held, step()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("B, H", [(30, 12), (37, 4), (128, 3), (129, 2)])
+def test_many_ragged_rows_in_any_order(B, H):
+    """More rows than SMs, ranked by length inside the kernel (up to 128 batch
+    rows): each row's bits are those it has on its own; every output is written."""
+
+    T, D = 400, 32
+    g = _gen(7)
+    lengths = torch.randint(0, T + 1, (B,), generator=g, device=DEV).to(torch.int32)
+    lengths[B // 2 :: 5] = 128  # ties
+    q, k, v, go = (_randn((T, B, H, D), s, torch.bfloat16) for s in (1, 2, 3, 5))
+    first = mb.DecayAttentionState(_randn((B, H, D, D), 4))
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    torch.full((T, B, H, D), float("nan"), dtype=torch.bfloat16, device=DEV)  # stale memory
+    state, out = mb.decay_attention_forward(*leaves, _decay(H), first, scale=0.2, lengths=lengths)
+    grads = torch.autograd.grad(out, leaves, go)
+    for b in range(0, B, 7):
+        own = [x[:, b : b + 1].contiguous().requires_grad_(True) for x in (q, k, v)]
+        s1, o1 = mb.decay_attention_forward(
+            *own, _decay(H), mb.DecayAttentionState(first.memory[b : b + 1]), scale=0.2,
+            lengths=lengths[b : b + 1])
+        g1 = torch.autograd.grad(o1, own, go[:, b : b + 1].contiguous())
+        assert torch.equal(out[:, b], o1[:, 0])
+        assert torch.equal(state.memory[b], s1.memory[0])
+        for x, y in zip(grads, g1):
+            assert torch.equal(x[:, b], y[:, 0])
+    live = _live(T, lengths)
+    for x in (out, *grads):
+        assert torch.equal(x.masked_fill(live, 0), torch.zeros_like(x))
