@@ -286,9 +286,8 @@ def _plain_int8(s):
     else:
         x = x.float()
         top = x.abs().amax(dim=1, keepdim=True)
-        levels = torch.full_like(top, 127.0)  # a tensor: divisions, not products by reciprocals
-        q = torch.round(x * torch.where(top > 0, levels / top, 0.0))
-        row_scale = top / levels
+        q = torch.round(x * torch.where(top > 0, 127.0 / top, 0.0))
+        row_scale = top / 127.0
     y = (q @ s["weight"].float().t()) * (row_scale * s["weight_scale"][None, :])
     return {"out": (y + s["bias"].float()).to(s["dtype"])}
 
