@@ -48,25 +48,50 @@ __device__ __forceinline__ T drop(T x, bool keep, float scale) {
   return Elem<T>::from_f(keep ? Elem<T>::to_f(x) * scale : 0.0f);
 }
 
+// A group's elements as pieces of BYTES bytes, each of which has to start on a multiple
+// of that: 16 (two pieces of fp32), or 32 for fp32 groups in one access.
+template <typename T, int BYTES>
+struct Group {
+  static constexpr int kPiece = BYTES / sizeof(T);
+  Vec<T, kPiece> piece[kGroup / kPiece];
+  __device__ __forceinline__ T& operator[](int j) { return piece[j / kPiece].v[j % kPiece]; }
+};
+
+template <typename T, int BYTES>
+__device__ __forceinline__ Group<T, BYTES> load_group(const T* p) {
+  constexpr int E = Group<T, BYTES>::kPiece;
+  Group<T, BYTES> g;
+#pragma unroll
+  for (int i = 0; i < kGroup / E; ++i) g.piece[i] = load_vec<T, E>(p + i * E);
+  return g;
+}
+
+template <typename T, int BYTES>
+__device__ __forceinline__ void store_group(T* p, const Group<T, BYTES>& g) {
+  constexpr int E = Group<T, BYTES>::kPiece;
+#pragma unroll
+  for (int i = 0; i < kGroup / E; ++i) store_vec<T, E>(p + i * E, g.piece[i]);
+}
+
 // Every element its own draw: kFlight groups per thread, a block's width apart, all
 // loads on their way before the generator runs. Bound by DRAM (4 bytes per 16-bit
 // element); the generator and the selects are about 110 issue slots per group, half
 // of what the copy bandwidth leaves. One group per thread, with the draws first made
-// into a bit mask, took 0.262 ms for 134 M bf16 elements.
+// into a bit mask, took 0.262 ms for 134 M bf16 elements. fp32 in 32-byte accesses where
+// both bases allow them (4 M elements in L2: 6.2 us, 8.3 in 16-byte ones; 67 M: 82 and 84).
 constexpr int kFlight = 4;
 
-template <typename T>
+template <typename T, int BYTES>
 __global__ void __launch_bounds__(kThreads)
     dropout_kernel(const T* __restrict__ x, T* __restrict__ y, int64_t n, uint32_t cut, float scale,
                    const int64_t* __restrict__ seed) {
-  using V = Vec<T, kGroup>;
   const int64_t groups = n / kGroup;
   const int64_t g0 = int64_t(blockIdx.x) * (kThreads * kFlight) + threadIdx.x;
-  V v[kFlight];
+  Group<T, BYTES> v[kFlight];
 #pragma unroll
   for (int i = 0; i < kFlight; ++i) {
     const int64_t g = g0 + i * kThreads;
-    if (g < groups) v[i] = load_vec<T, kGroup>(x + g * kGroup);
+    if (g < groups) v[i] = load_group<T, BYTES>(x + g * kGroup);
   }
   const uint64_t key = static_cast<uint64_t>(seed[0]), offset = static_cast<uint64_t>(seed[1]);
 #pragma unroll
@@ -75,19 +100,19 @@ __global__ void __launch_bounds__(kThreads)
     if (g >= groups) return;
     const Words r = philox(static_cast<uint64_t>(g), offset, key);
 #pragma unroll
-    for (int j = 0; j < kGroup; ++j) v[i].v[j] = drop(v[i].v[j], kept(r, j, cut), scale);
-    store_vec<T, kGroup>(y + g * kGroup, v[i]);
+    for (int j = 0; j < kGroup; ++j) v[i][j] = drop(v[i][j], kept(r, j, cut), scale);
+    store_group<T, BYTES>(y + g * kGroup, v[i]);
   }
 }
 
 // One mask for `rows` rows, and any alignment: a thread owns one group of the n
-// elements and walks the rows [row0, row1), four in flight.
+// elements and walks the rows [row0, row1), four in flight. fp32 in 16-byte accesses
+// whatever the alignment (256 rows of 262144: 86 us, 103 in 32-byte ones).
 template <typename T, bool VECTOR>
 __global__ void __launch_bounds__(kThreads)
     dropout_rows_kernel(const T* __restrict__ x, T* __restrict__ y, int64_t rows, int64_t n,
                         int64_t rows_per_block, uint32_t cut, float scale,
                         const int64_t* __restrict__ seed) {
-  using V = Vec<T, kGroup>;
   const int64_t groups = (n + kGroup - 1) / kGroup;
   const int64_t g = int64_t(blockIdx.x) * kThreads + threadIdx.x;
   if (g >= groups) return;
@@ -96,10 +121,10 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t e0 = g * kGroup;
   const uint64_t key = static_cast<uint64_t>(seed[0]), offset = static_cast<uint64_t>(seed[1]);
   if constexpr (VECTOR) {
-    V v[kFlight];
+    Group<T, 16> v[kFlight];
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
-      if (row0 + i < row1) v[i] = load_vec<T, kGroup>(x + (row0 + i) * n + e0);
+      if (row0 + i < row1) v[i] = load_group<T, 16>(x + (row0 + i) * n + e0);
     }
     const Words r = philox(static_cast<uint64_t>(g), offset, key);
     bool keep[kGroup];
@@ -109,11 +134,11 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int i = 0; i < kFlight; ++i) {
         if (row + i >= row1) break;
-        V out;
+        Group<T, 16> out;
 #pragma unroll
-        for (int j = 0; j < kGroup; ++j) out.v[j] = drop(v[i].v[j], keep[j], scale);
-        if (row + i + kFlight < row1) v[i] = load_vec<T, kGroup>(x + (row + i + kFlight) * n + e0);
-        store_vec<T, kGroup>(y + (row + i) * n + e0, out);
+        for (int j = 0; j < kGroup; ++j) out[j] = drop(v[i][j], keep[j], scale);
+        if (row + i + kFlight < row1) v[i] = load_group<T, 16>(x + (row + i + kFlight) * n + e0);
+        store_group<T, 16>(y + (row + i) * n + e0, out);
       }
     }
   } else {
@@ -136,13 +161,15 @@ int launch(const void* x, void* y, int64_t rows, int64_t n, int threshold, const
   T* ys = static_cast<T*>(y);
   const float scale = 65536.0f / static_cast<float>(65536 - threshold);
   const uint32_t cut = static_cast<uint32_t>(threshold) << 16;
+  static_assert(alignof(Group<T, 16>) == 16 && alignof(Group<float, 32>) == 32, "accesses");
   const bool vector = n % kGroup == 0 && aligned_to(x, 16) && aligned_to(y, 16);
+  const bool wide = sizeof(T) == 4 && aligned_to(x, 32) && aligned_to(y, 32);
   const int64_t groups = ceil_div(n, kGroup);
   if (rows == 1 && vector) {
     const int64_t blocks = ceil_div(groups, kThreads * kFlight);
     MB_CHECK_ARG(blocks <= 0x7fffffff, "mb_dropout: too many elements");
-    dropout_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(xs, ys, n, cut,
-                                                                              scale, seed);
+    auto kern = wide ? dropout_kernel<T, 8 * sizeof(T)> : dropout_kernel<T, 16>;
+    kern<<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(xs, ys, n, cut, scale, seed);
   } else {
     const int64_t bx = ceil_div(groups, kThreads);
     MB_CHECK_ARG(bx <= 0x7fffffff, "mb_dropout: too many elements");
