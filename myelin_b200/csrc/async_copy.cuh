@@ -133,6 +133,16 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   return false;
 }
 
+// The waits of a thread whose warp works as a whole (tensor-memory loads, warp and named
+// barriers: leaving early would strand the others). When one runs out, which is recorded,
+// the later ones return at once and the thread goes on to its end, on whatever is there.
+struct Waits {
+  bool over = false;
+  __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) {
+    if (!over) over = !mbar_wait_bounded(bar, parity);
+  }
+};
+
 namespace {
 
 // Diagnostic: one thread waits, with a poll budget of `polls`, for phase 0 of

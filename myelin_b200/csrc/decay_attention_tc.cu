@@ -704,20 +704,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int r = quarter * 32 + lane;
     const float intra = a.out_scale * a.kv_scale;
     uint32_t it = 0, hand = 0;
-    bool ok = true;
-    for (uint32_t unit = blockIdx.x; unit < visits && ok; unit += gridDim.x) {
+    Waits wait;
+    for (uint32_t unit = blockIdx.x; unit < visits; unit += gridDim.x) {
       const Unit u = decode_unit(args, unit, order);
       for (int i = 0; i < u.chunks; ++i, ++it) {
         const int s = it & 1;
         const int n = chunk_steps(u, chunk_t0(u, i, reverse));
         const uint32_t t_scores = tmem + L::kScores + s * 128 + (uint32_t(quarter * 32) << 16);
-        ok = false;
-        if (!mbar_wait_bounded(&full_k[s], (it >> 1) & 1)) break;
-        if (!mbar_wait_bounded(&scores_done[s], (it >> 1) & 1)) break;
+        wait(&full_k[s], (it >> 1) & 1);
+        wait(&scores_done[s], (it >> 1) & 1);
         if (n < kC) {
           // (with one V stage these warps may be here before the last chunk left it)
-          if (VS == 1 && it >= 1 && !mbar_wait_bounded(out_done, (it - 1) & 1)) break;
-          if (!mbar_wait_bounded(&full_v[it % VS], (it / VS) & 1)) break;
+          if (VS == 1 && it >= 1) wait(out_done, (it - 1) & 1);
+          wait(&full_v[it % VS], (it / VS) & 1);
           if (r >= n) zero_v_row<DV>(smem + L::kV + (it % VS) * L::kVBytes, r, half);
           fence_proxy_async_smem();
         }
@@ -788,14 +787,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (i + 1 < u.chunks) {
           // K <- W_kv K (the scores that read K are complete), and what rounding leaves
           // of it, once the last chunk's remainders are used
-          if (hand >= 1 && !mbar_wait_bounded(delta_done, (hand - 1) & 1)) break;
+          if (hand >= 1) wait(delta_done, (hand - 1) & 1);
           ++hand;
           weigh_k_row<T, DK, 2>(smem + L::kK + s * L::kQBytes, smem + L::kLo, r, half,
                                 r < n ? kv_weight(u, r, n, reverse) : 0.0f, r < n);
           fence_proxy_async_smem();
           warp_arrive(kw_ready, lane);
         }
-        ok = true;
       }
     }
   } else {
@@ -846,8 +844,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       warp_arrive(carry_ready, lane);
     };
     uint32_t it = 0, hand = 0;
-    bool ok = true;
-    for (uint32_t unit = blockIdx.x; unit < visits && ok; unit += gridDim.x) {
+    Waits wait;
+    for (uint32_t unit = blockIdx.x; unit < visits; unit += gridDim.x) {
       const Unit u = decode_unit(args, unit, order);
       T* o = static_cast<T*>(a.o.data) + u.b * a.o.stride_b + u.h * a.o.stride_h;
       if (u.chunks > 0) {
@@ -871,7 +869,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int64_t t0 = chunk_t0(u, i, reverse);
         const int n = chunk_steps(u, t0);
         const int s = it & 1;
-        ok = false;
         const float inv_now = inv_s;  // of the operand behind this chunk's Q S
         auto release = [&]() {  // the last chunk's Q stage: its outputs have left it
           if (L::kFull && owed && lane == 0) {
@@ -882,7 +879,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         };
         if (i + 1 < u.chunks) {
           release();
-          if (!mbar_wait_bounded(delta_done, hand & 1)) break;
+          wait(delta_done, hand & 1);
           ++hand;
           tc_fence_after();
           if (holds) {
@@ -901,7 +898,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           put_carry();
         }
         release();
-        if (!mbar_wait_bounded(out_done, it & 1)) break;
+        wait(out_done, it & 1);
         tc_fence_after();
         const float w_in = kHalf ? row_scale[s * kC + r] : 1.0f;
         const bool inter = i > 0 || carry_in;
@@ -963,7 +960,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (L::kFull) tma_store_wait_read<0>();
           mbar_arrive(&empty_q[s]);
         }
-        ok = true;
       }
       if (u.chunks < 0) continue;
       // whole chunks past the row's length: zeros
@@ -1102,27 +1098,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const int r = quarter * 32 + lane;
     uint32_t it = 0;
-    bool ok = true;
-    for (uint32_t unit = blockIdx.x; unit < visits && ok; unit += gridDim.x) {
+    Waits wait;
+    for (uint32_t unit = blockIdx.x; unit < visits; unit += gridDim.x) {
       const Unit u = decode_unit(args, unit, order);
       for (int i = 0; i < u.chunks; ++i, ++it) {
         const int s = it & 1;
         const int n = chunk_steps(u, chunk_t0(u, i, reverse));
         uint8_t* ks = smem + L::kK + s * L::kKBytes;
-        ok = false;
-        if (!mbar_wait_bounded(&full_k[s], (it >> 1) & 1)) break;
+        wait(&full_k[s], (it >> 1) & 1);
         if (n < kC) {
-          if (!mbar_wait_bounded(&full_v[s], (it >> 1) & 1)) break;
+          wait(&full_v[s], (it >> 1) & 1);
           if (r >= n) zero_v_row<DV>(smem + L::kV + s * L::kVBytes, r, half);
         }
         // the further parts' buffers are free once the last chunk's products are
         // complete; the two halves of a chunk's steps go through on their own
-        if (it >= 1 && !mbar_wait_bounded(&kw_used[r >> 6], (it - 1) & 1)) break;
+        if (it >= 1) wait(&kw_used[r >> 6], (it - 1) & 1);
         weigh_k_row<T, DK, PARTS>(ks, smem + L::kLo, r, half,
                                   r < n ? kv_weight(u, r, n, reverse) : 0.0f, r < n);
         fence_proxy_async_smem();
         warp_arrive(&kw_ready[r >> 6], lane);
-        ok = true;
       }
     }
   } else {
@@ -1134,8 +1128,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const bool holds = quarter * 32 < DK;
     const bool row_ok = r < a.Dk && col0 < a.Dv;
     uint32_t it = 0;
-    bool ok = true;
-    for (uint32_t unit = blockIdx.x; unit < visits && ok; unit += gridDim.x) {
+    Waits wait;
+    for (uint32_t unit = blockIdx.x; unit < visits; unit += gridDim.x) {
       const Unit u = decode_unit(args, unit, order);
       if (u.chunks < 0) continue;
       float S[kCols];
@@ -1159,9 +1153,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       load_memory_row<kCols>(from, from_sc, a.Dv - col0, S);
       for (int i = 0; i < u.chunks; ++i, ++it) {
         const int n = chunk_steps(u, chunk_t0(u, i, reverse));
-        ok = false;
         // (the second half's products come after the first's)
-        if (!mbar_wait_bounded(&kw_used[1], it & 1)) break;
+        wait(&kw_used[1], it & 1);
         tc_fence_after();
         if (holds) {
           const float gn = decay_pow(u.log2g, n);
@@ -1178,9 +1171,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         tc_fence_before();
         warp_arrive(delta_read, lane);
-        ok = true;
       }
-      if (!ok) break;
       if (args.m_map) {
         // whole 128-byte rows by tensor stores, 32 x 32 values at a time (a lane's own
         // row-wise stores touch 32 lines per instruction)

@@ -617,6 +617,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     const int quarter = warp & 3;
     uint8_t* slot = sslot + (warp - 2) * L::kSlotBytes;
     float2* cols = reinterpret_cast<float2*>(scol + (warp - 2) * L::kColBytes);
+    Waits wait;
     uint32_t local = 0;
     for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++local) {
       const uint32_t b = local & 1;
@@ -625,7 +626,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       __syncwarp();  // the previous tile's column scales have been read
       load_cols<BN>(cols, col0, lane, args);
       const float s_row = row_a_scale(args, row0 + lane);
-      if (!mbar_wait_bounded(&acc_full[b], (local >> 1) & 1)) break;
+      wait(&acc_full[b], (local >> 1) & 1);
       tc_fence_after();
       drain_i8<TOut, BN>(tmem_base + (uint32_t(quarter * 32) << 16) + b * BN, row0, col0, lane,
                          args, &tma_c, s_row, cols, slot);
@@ -778,6 +779,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8PairThreads, 1)
     const int half = (warp - 2) >> 2;
     uint8_t* slot = sslot + (warp - 2) * L::kSlotBytes;
     float2* cols = reinterpret_cast<float2*>(scol + (warp - 2) * L::kColBytes);
+    Waits wait;
     uint32_t local = 0;
     for (int64_t tile = pair; tile < tiles; tile += pairs, ++local) {
       const uint32_t b = local & 1;
@@ -786,7 +788,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8PairThreads, 1)
       __syncwarp();  // the previous tile's column scales have been read
       load_cols<128>(cols, col0, lane, args);
       const float s_row = row_a_scale(args, row0 + lane);
-      if (!mbar_wait_bounded(&acc_full[b], (local >> 1) & 1)) break;
+      wait(&acc_full[b], (local >> 1) & 1);
       tc_fence_after();
       drain_i8<TOut, 128>(tmem_base + (uint32_t(quarter * 32) << 16) + b * 256 + half * 128, row0,
                           col0, lane, args, &tma_c, s_row, cols, slot);

@@ -432,6 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool use_tma = args.tma_store != 0;
     uint8_t* slots = sepi + (warp - 2) * 2 * L::kEpiSlotBytes;
     uint32_t nstore = 0;
+    Waits wait;
     uint32_t local = 0;
     for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x, ++local) {
       const uint32_t b = local & 1;
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t tn = wu.tile % n_tiles;
       float bcol[BN / 32];
       load_bias_cols(args, tn * BN, lane, bcol);
-      if (!mbar_wait_bounded(&acc_full[b], (local >> 1) & 1)) break;
+      wait(&acc_full[b], (local >> 1) & 1);
       tc_fence_after();
       const DrainTarget tgt{&tma_c, args.k_slices > 1, args.bias != nullptr, 0};
       drain_tile<TOut, BN>(tmem_base + (uint32_t(quarter * 32) << 16) + b * BN,
@@ -687,6 +688,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(k2Threads, 1)
     const bool use_tma = args.tma_store != 0;
     uint8_t* slots = sepi + (warp - 2) * L::kEpiWarpBytes;
     uint32_t nstore = 0;
+    Waits wait;
     uint32_t local = 0;
     for (int64_t unit = pair; unit < units; unit += pairs, ++local) {
       const uint32_t b = local & 1;
@@ -698,7 +700,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(k2Threads, 1)
       const int64_t row0 = tm * k2BM + int64_t(rank) * 128 + quarter * 32;
       float bcol[k2BN / 2 / 32];
       load_bias_cols(args, col_tile0, lane, bcol);
-      if (!mbar_wait_bounded(&acc_full[b], (local >> 1) & 1)) break;
+      wait(&acc_full[b], (local >> 1) & 1);
       tc_fence_after();
       if (wu.partial) {
         // a slice of a tail tile: fp32 partial sums to the workspace (no bias)
