@@ -11,7 +11,15 @@
 
 namespace mb {
 
+// The driver's function works in the calling thread's current context. A thread that has
+// made no CUDA call yet has none (the autograd engine's, at a process's first backward
+// pass), so its device is set once, which makes that device's context current.
 inline PFN_cuTensorMapEncodeTiled_v12000 tma_encode_fn() {
+  static thread_local bool bound = false;
+  if (!bound) {
+    int device = 0;
+    bound = cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess;
+  }
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
