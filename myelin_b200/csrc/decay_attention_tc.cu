@@ -5,10 +5,12 @@
 //
 //   outputs  P = (Q K^T) * g^|r-j| on the causal side    O = P V + W_out (Q S)
 //            D = (W_kv K)^T V                             S <- g^n S + c D
-//   states   D and S only, with W_kv K in two (fp16) or three (bf16) 16-bit parts
-//            whose sum keeps all its bits: the memories that leave the operator
-//            are good to fp32, while the carry inside the outputs kernel, which is
-//            rounded to 16 bits before use, takes one part.
+//   states   D and S only
+//
+// W_kv K goes as 16-bit parts whose sum keeps its bits: in the states kernel two of fp16
+// (brought to a common magnitude by a power of two first, which leaves 2^-22) or three of
+// bf16, so that the memories that leave the operator are good to fp32; in the outputs
+// kernel two of either, since the carry there is rounded to 16 bits before use.
 //
 // All products are tcgen05 (M = 128 steps or memory rows, sums in TMEM). 20 warps:
 //   warp 0      copies: Q, K, V, two stages of 128-byte-swizzled tiles
@@ -77,7 +79,9 @@ struct OutLayout {
                                                           // P's rows, by stage
   static constexpr int kRowTop = kRowScale + 2 * kC * 4;  // fp16: largest of the other half
   static constexpr int kMax = kRowTop + kC * 4;           // fp16: largest values of each warp
-  static constexpr int kBars = kMax + 2 * 8 * 4;
+  static constexpr int kKeyTop = kMax + 2 * 8 * 4;        // fp16: largest weighed key of each warp
+  static constexpr int kKeyInv = kKeyTop + 2 * 8 * 4;     // fp16: 1 / scale of the weighed keys
+  static constexpr int kBars = kKeyInv + 2 * 4;
   static constexpr int kNumBars = 20;
   static constexpr int kOrder = kBars + kNumBars * 8 + 16;  // batch rows, longest first
   static constexpr size_t kSmem = kOrder + kMaxOrder * 2;
@@ -98,11 +102,13 @@ struct StatesLayout {
   static constexpr int kLo = kK + 2 * kKBytes;  // the further parts of W_kv K
   static constexpr int kV = kLo + (PARTS - 1) * kKBytes;
   static constexpr int kOut = kV + 2 * kVBytes;  // 32 x 32 fp32 per carry warp, on the way out
-  static constexpr int kBars = kOut + 8 * 4096;
+  static constexpr int kKeyTop = kOut + 8 * 4096;      // fp16: largest weighed key of each warp
+  static constexpr int kKeyInv = kKeyTop + 2 * 8 * 4;  // fp16: 1 / scale of the weighed keys
+  static constexpr int kBars = kKeyInv + 2 * 4;
   static constexpr int kNumBars = 12;
   static constexpr int kOrder = kBars + kNumBars * 8 + 16;  // batch rows, longest first
   static constexpr size_t kSmem = kOrder + kMaxOrder * 2;
-  static_assert(kSmem <= 232448, "shared memory");
+  static_assert(kBars % 8 == 0 && kSmem <= 232448, "shared memory");
   static constexpr uint32_t kDelta = 0;
 };
 
@@ -332,7 +338,7 @@ __device__ __forceinline__ float fp16_scale(float top) {
 }
 
 // Named barriers: 2 the carry warps, 3..6 the two score warps and 7..10 the two
-// output warps of one TMEM lane quarter.
+// output warps of one TMEM lane quarter, 11 the warps that weigh the keys.
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -370,6 +376,34 @@ __device__ __forceinline__ void weigh_k_row(uint8_t* ks, uint8_t* lo, int r, int
       *reinterpret_cast<uint4*>(to + at) = make_uint4(y[0], y[1], y[2], y[3]);
     }
   }
+}
+
+// fp16: the power of two that brings a chunk's largest weighed key to [2^13, 2^14), so
+// that two parts leave 2^-22 of a key whatever the keys' magnitude (rounded where they
+// are, keys of 1e-5 lost 0.5 %, since the second part adds nothing below 2^-24). One for
+// the whole chunk, whose products are one sum. `tops` has 8 values for each of two chunks:
+// who writes a chunk's has passed the barrier of the one between.
+template <int DK>
+__device__ __forceinline__ float key_scale(const uint8_t* ks, float* tops, int r, int half,
+                                           float w, bool valid) {
+  __half2 top2 = __float2half2_rn(0.0f);
+#pragma unroll
+  for (int q = 0; q < DK / 16; ++q) {
+    const uint4 x = *reinterpret_cast<const uint4*>(ks + piece_at(r, half * (DK / 16) + q, kC));
+    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      top2 = __hmax2(top2, __habs2(*reinterpret_cast<const __half2*>(&in[e])));
+    }
+  }
+  const float mine = valid ? w * __half2float(__hmax(__low2half(top2), __high2half(top2))) : 0.0f;
+  const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(mine));
+  if ((threadIdx.x & 31) == 0) tops[(threadIdx.x >> 5) - 4] = __uint_as_float(top);
+  bar_sync(11, kGroup);
+  float all = tops[0];
+#pragma unroll
+  for (int x = 1; x < 8; ++x) all = fmaxf(all, tops[x]);
+  return fp16_scale(all);
 }
 
 template <int N>
@@ -490,6 +524,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   float* row_scale = reinterpret_cast<float*>(smem + L::kRowScale);
   float* row_top = reinterpret_cast<float*>(smem + L::kRowTop);
   float* warp_max = reinterpret_cast<float*>(smem + L::kMax);
+  float* key_top = reinterpret_cast<float*>(smem + L::kKeyTop);
+  float* key_inv = reinterpret_cast<float*>(smem + L::kKeyInv);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
   uint64_t* full_q = bars;            // [2]
   uint64_t* full_k = bars + 2;        // [2]
@@ -526,7 +562,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_init(out_done, 2);  // the products' completion, and what their operands' makers wrote
     mbar_init(out_read, 8);
     mbar_init(kw_ready, 8);
-    mbar_init(delta_done, 1);
+    mbar_init(delta_done, kHalf ? 2 : 1);  // fp16: with the scale that the keys' weighers wrote
     mbar_init(carry_ready, 8);
     mbar_init(drained, 1);
     fence_barrier_init();
@@ -673,6 +709,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               mma_f16(tmem + L::kDelta, k0 + k * 128, v0 + k * 128, i_delta, 1u);
             }
             mma_commit(delta_done);
+            if (kHalf) mbar_arrive(delta_done);
             if (scored == it + 1 && !scores(it + 1, false)) break;
             // D has been read: its columns take P V
             if (!mbar_wait_bounded(carry_ready, cin & 1)) break;
@@ -787,10 +824,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (i + 1 < u.chunks) {
           // K <- W_kv K (the scores that read K are complete), and what rounding leaves
           // of it, once the last chunk's remainders are used
+          uint8_t* ks = smem + L::kK + s * L::kQBytes;
+          float w = r < n ? kv_weight(u, r, n, reverse) : 0.0f;
+          float k_scale = 1.0f;
+          if constexpr (kHalf) k_scale = key_scale<DK>(ks, key_top + (hand & 1) * 8, r, half, w, r < n);
           if (hand >= 1) wait(delta_done, (hand - 1) & 1);
+          if (kHalf && threadIdx.x == 4 * 32) key_inv[hand & 1] = 1.0f / k_scale;
           ++hand;
-          weigh_k_row<T, DK, 2>(smem + L::kK + s * L::kQBytes, smem + L::kLo, r, half,
-                                r < n ? kv_weight(u, r, n, reverse) : 0.0f, r < n);
+          weigh_k_row<T, DK, 2>(ks, smem + L::kLo, r, half, w * k_scale, r < n);
           fence_proxy_async_smem();
           warp_arrive(kw_ready, lane);
         }
@@ -880,6 +921,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (i + 1 < u.chunks) {
           release();
           wait(delta_done, hand & 1);
+          const float d_scale = kHalf ? a.kv_scale * key_inv[hand & 1] : a.kv_scale;
           ++hand;
           tc_fence_after();
           if (holds) {
@@ -891,7 +933,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tmem_wait_ld();
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
-                S[c0 + j] = fmaf(gn, S[c0 + j], a.kv_scale * __uint_as_float(x[j]));
+                S[c0 + j] = fmaf(gn, S[c0 + j], d_scale * __uint_as_float(x[j]));
               }
             }
           }
@@ -986,9 +1028,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                        const __grid_constant__ CUtensorMap map_m,
                        const __grid_constant__ TcArgs args) {
   constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
+  constexpr bool kHalf = std::is_same<T, __half>::value;
   using L = StatesLayout<DK, DV, PARTS>;
   constexpr int kCols = DV / 2;
   extern __shared__ __align__(1024) uint8_t smem[];
+  float* key_top = reinterpret_cast<float*>(smem + L::kKeyTop);
+  float* key_inv = reinterpret_cast<float*>(smem + L::kKeyInv);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
   uint64_t* full_k = bars;      // [2]
   uint64_t* full_v = bars + 2;  // [2]
@@ -1010,7 +1055,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&full_v[s], 1);
       mbar_init(&empty[s], 1);
       mbar_init(&kw_ready[s], 4);
-      mbar_init(&kw_used[s], 1);
+      // fp16: the second with the scale that the keys' weighers wrote
+      mbar_init(&kw_used[s], kHalf && s == 1 ? 2 : 1);
     }
     mbar_init(delta_read, 8);
     mbar_init(drained, 1);
@@ -1084,6 +1130,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               }
             }
             mma_commit(&kw_used[x]);
+            if (kHalf && x == 1) mbar_arrive(&kw_used[x]);
             ok = x == 1;
           }
           if (!ok) break;
@@ -1110,11 +1157,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           wait(&full_v[s], (it >> 1) & 1);
           if (r >= n) zero_v_row<DV>(smem + L::kV + s * L::kVBytes, r, half);
         }
+        float w = r < n ? kv_weight(u, r, n, reverse) : 0.0f;
+        float k_scale = 1.0f;
+        if constexpr (kHalf) k_scale = key_scale<DK>(ks, key_top + s * 8, r, half, w, r < n);
         // the further parts' buffers are free once the last chunk's products are
         // complete; the two halves of a chunk's steps go through on their own
         if (it >= 1) wait(&kw_used[r >> 6], (it - 1) & 1);
-        weigh_k_row<T, DK, PARTS>(ks, smem + L::kLo, r, half,
-                                  r < n ? kv_weight(u, r, n, reverse) : 0.0f, r < n);
+        // (the last chunk but one's has been read: its sums left the accumulator before
+        // the last chunk's second half was issued)
+        if (kHalf && threadIdx.x == 6 * 32) key_inv[s] = 1.0f / k_scale;
+        weigh_k_row<T, DK, PARTS>(ks, smem + L::kLo, r, half, w * k_scale, r < n);
         fence_proxy_async_smem();
         warp_arrive(&kw_ready[r >> 6], lane);
       }
@@ -1155,6 +1207,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int n = chunk_steps(u, chunk_t0(u, i, reverse));
         // (the second half's products come after the first's)
         wait(&kw_used[1], it & 1);
+        const float d_scale = kHalf ? a.kv_scale * key_inv[it & 1] : a.kv_scale;
         tc_fence_after();
         if (holds) {
           const float gn = decay_pow(u.log2g, n);
@@ -1165,7 +1218,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tmem_wait_ld();
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              S[c0 + j] = fmaf(gn, S[c0 + j], a.kv_scale * __uint_as_float(x[j]));
+              S[c0 + j] = fmaf(gn, S[c0 + j], d_scale * __uint_as_float(x[j]));
             }
           }
         }
