@@ -684,6 +684,35 @@ def dropout(x: torch.Tensor, seed: torch.Tensor, threshold: int,
     return dropout_op(*args) if _tracing() else _dropout_impl(*args)
 
 
+def _next_seed_impl(rng: torch.Tensor) -> torch.Tensor:
+    # Inside a backward pass this can only be a forward that runs again (activation
+    # checkpointing), whose first run drew an earlier offset.
+    if torch._C._current_graph_task_id() != -1:
+        raise RuntimeError(
+            "dropout was run again inside a backward pass and would draw another mask than its "
+            "forward did; take the seed outside what is checkpointed (seed = "
+            "dropout.next_seed()) and pass it as an argument"
+        )
+    seed = rng.clone()
+    rng[1:].add_(1)
+    return seed
+
+
+next_seed_op = torch.library.custom_op(f"{_NS}::next_seed", _next_seed_impl,
+                                       mutates_args=("rng",))
+
+
+@next_seed_op.register_fake
+def _next_seed_fake(rng):
+    return rng.new_empty(rng.shape)
+
+
+def next_seed(rng: torch.Tensor) -> torch.Tensor:
+    """``rng`` (seed, calls so far) as this call's seed; counts the call in place."""
+
+    return next_seed_op(rng) if _tracing() else _next_seed_impl(rng)
+
+
 # ---------------------------------------------------------------------------
 # projection in 8-bit integers
 # ---------------------------------------------------------------------------
@@ -773,5 +802,5 @@ def quantized_project(x2: torch.Tensor, x_scale: torch.Tensor | None, weight: to
 OPS = (scan_forward_op, scan_backward_op, gemm_tn_op, linear_project_op, linear_input_grad_op,
        linear_weight_grad_op, bias_grad_op, pack_op, unpack_op, count_rows_op, count_columns_op,
        pack_count_op, izhikevich_op, decay_attention_op, decay_attention_backward_op,
-       decay_attention_step_op, decay_attention_step_inplace_op, dropout_op, quantize_rows_op,
+       decay_attention_step_op, decay_attention_step_inplace_op, dropout_op, next_seed_op, quantize_rows_op,
        quantized_project_op)

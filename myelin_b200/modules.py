@@ -22,7 +22,7 @@ from myelin_b200.attention import (
     decay_attention_step,
 )
 from myelin_b200.checkpointing import CheckpointSize
-from myelin_b200.compile_ops import i8_operand
+from myelin_b200.compile_ops import i8_operand, next_seed
 from myelin_b200.dropout import spike_dropout
 from myelin_b200.kernels import (
     izhikevich_step,
@@ -374,6 +374,15 @@ class SpikeDropout(nn.Module):
     module; each call in training mode takes the next offset on the device, so a
     captured graph draws a new mask at every replay. With ``time_shared`` (the
     default) all steps of a ``[T, ...]`` input use one mask.
+
+    A call that activation checkpointing runs again in the backward pass has to draw
+    the same mask: take its seed first and pass it,
+    ``checkpoint(dropout, x, dropout.next_seed())``. Without one the second run is
+    refused. A copy of the module (``copy.deepcopy``) draws the same masks as the
+    original, and a wrapper that broadcasts buffers from rank 0 (as
+    ``DistributedDataParallel`` does) makes all ranks draw the same: where they
+    should differ, give each its own first word, ``dropout.rng[0] = ...``, and keep
+    the buffer out of the broadcast.
     """
 
     def __init__(self, p: float = 0.5, *, time_shared: bool = True,
@@ -385,17 +394,31 @@ class SpikeDropout(nn.Module):
         self.time_shared = time_shared
         first = int(torch.randint(2**62, ())) if seed is None else seed
         self.register_buffer("rng", torch.tensor([first, 0], dtype=torch.int64))
-        self.register_buffer("_next", torch.tensor([0, 1], dtype=torch.int64), persistent=False)
 
-    def forward(self, inputs: torch.Tensor) -> torch.Tensor:
+    def next_seed(self) -> torch.Tensor:
+        """The (seed, offset) of the next call, which is then counted as made."""
+
+        return next_seed(self.rng)
+
+    def forward(self, inputs: torch.Tensor, seed: torch.Tensor | None = None) -> torch.Tensor:
+        """With ``seed`` (from ``next_seed``) the mask is that seed's and no call is counted."""
+
         if not self.training or self.p == 0.0:
             return inputs
-        seed = self.rng.clone()  # this call's own: its backward draws from it again
-        self.rng.add_(self._next)
+        if seed is None:
+            seed = self.next_seed()  # this call's own: its backward draws from it again
         return spike_dropout(inputs, self.p, seed, time_shared=self.time_shared)
 
     def extra_repr(self) -> str:
         return f"p={self.p}, time_shared={self.time_shared}"
+
+
+def _drop(dropout: nn.Module, inputs: torch.Tensor, seed: torch.Tensor | None) -> torch.Tensor:
+    if seed is None:
+        return dropout(inputs)
+    if not isinstance(dropout, SpikeDropout):
+        raise ValueError(f"dropout_seed needs a SpikeDropout; got {type(dropout).__name__}")
+    return dropout(inputs, seed)
 
 
 class DecayAttention(nn.Module):
@@ -407,7 +430,8 @@ class DecayAttention(nn.Module):
     ``LIFParams.decay``). ``forward`` takes ``[T, B, in_features]`` and carries the
     memories from ``initial_state`` to the state it returns; ``step`` takes one
     time step ``[B, in_features]``. Dropout (``SpikeDropout``, one mask for all
-    steps) applies in training mode, in ``forward`` only.
+    steps) applies in training mode, in ``forward`` only; under activation
+    checkpointing pass ``dropout_seed=layer.dropout.next_seed()``.
     """
 
     def __init__(
@@ -459,11 +483,12 @@ class DecayAttention(nn.Module):
         inputs: torch.Tensor,
         initial_state: DecayAttentionState | None = None,
         lengths: torch.Tensor | None = None,
+        dropout_seed: torch.Tensor | None = None,
     ) -> tuple[DecayAttentionState, torch.Tensor]:
         q, k, v = self._heads(inputs)
         state, out = decay_attention_forward(q, k, v, self.decay, initial_state,
                                              scale=self.key_size**-0.5, lengths=lengths)
-        return state, self.output(self.dropout(out.flatten(-2)))
+        return state, self.output(_drop(self.dropout, out.flatten(-2), dropout_seed))
 
     def step(
         self,
@@ -483,7 +508,8 @@ class RateReadoutClassifier(nn.Module):
     """Hidden streamed LIF layer plus a rate readout (src/myelin/modules.py:848-903).
 
     ``time_shared_dropout`` drops hidden neurons for the whole window
-    (``SpikeDropout``) instead of per step (``nn.Dropout``).
+    (``SpikeDropout``) instead of per step (``nn.Dropout``); under activation
+    checkpointing pass ``dropout_seed=net.dropout.next_seed()`` with it.
     """
 
     def __init__(
@@ -529,8 +555,10 @@ class RateReadoutClassifier(nn.Module):
             reduction="none",
         )
 
-    def forward(self, inputs: torch.Tensor) -> torch.Tensor:
-        hidden_spikes = self.dropout(self.hidden(inputs))
+    def forward(
+        self, inputs: torch.Tensor, dropout_seed: torch.Tensor | None = None
+    ) -> torch.Tensor:
+        hidden_spikes = _drop(self.dropout, self.hidden(inputs), dropout_seed)
         return self.output(hidden_spikes)
 
 
