@@ -20,7 +20,7 @@ import torch
 
 from myelin_b200 import _native as nat
 from myelin_b200 import compile_ops as cops
-from myelin_b200.autograd import DecayAttentionFunction
+from myelin_b200.autograd import DecayAttentionFunction, refuse_tangents, wants_grad
 
 MAX_HEAD_SIZE = 256
 
@@ -137,10 +137,8 @@ def decay_attention_forward(
             raise ValueError("lengths must be int32 on the same device as queries")
         lengths = lengths.contiguous()
     decay = decay.contiguous()
-    if torch.is_grad_enabled() and (
-        queries.requires_grad or keys.requires_grad or values.requires_grad
-        or (memory is not None and memory.requires_grad)
-    ):
+    refuse_tangents("decayed attention", queries, keys, values, memory, decay)
+    if wants_grad(queries, keys, values, memory):
         out, last = DecayAttentionFunction.apply(queries, keys, values, decay, memory, lengths,
                                                  float(scale))
     else:
@@ -179,16 +177,16 @@ def decay_attention_step(
             raise ValueError("active must be bool on the same device as query")
         active = active.contiguous()
     decay = decay.contiguous()
-    wants_grad = torch.is_grad_enabled() and any(
-        t.requires_grad for t in (query, key, value, memory))
+    refuse_tangents("decayed attention", query, key, value, memory, decay)
+    graph = wants_grad(query, key, value, memory)
     if inplace:
-        if wants_grad:
+        if graph:
             raise ValueError("inplace=True cannot be differentiated; use inplace=False")
         if not memory.is_contiguous():
             raise ValueError("inplace=True needs a contiguous state.memory")
         out = cops.decay_attention_step_(query, key, value, decay, memory, active, scale)
         return state, out
-    if wants_grad:
+    if graph:
         lengths = None if active is None else active.to(torch.int32)
         last, out = decay_attention_forward(
             query.unsqueeze(0), key.unsqueeze(0), value.unsqueeze(0), decay, state, scale=scale,

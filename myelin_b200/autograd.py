@@ -285,6 +285,23 @@ class TwoLayerPackedHiddenRateFunction(torch.autograd.Function):
         return (grad_x, grad_w1, grad_b1, grad_w2, grad_b2, *tail)
 
 
+def wants_grad(*tensors: torch.Tensor | None) -> bool:
+    """Whether a gradient is asked for."""
+
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Raise where a tensor carries a forward-mode tangent: a launch would drop it, and
+    the derivative would read as zero."""
+
+    forward = torch.autograd.forward_ad
+    if forward._current_level >= 0 and any(
+        t is not None and forward.unpack_dual(t).tangent is not None for t in tensors
+    ):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 class DecayAttentionFunction(torch.autograd.Function):
     """Attention with a decay for each head: (queries, keys, values, memory) ->
     (outputs, final memory). Saves its inputs only; the backward runs the same
@@ -305,6 +322,7 @@ class DecayAttentionFunction(torch.autograd.Function):
     def backward(ctx: Any, g_out, g_last):
         if g_out is None and g_last is None:
             return (None,) * 7
+        refuse_tangents("the gradient of decayed attention", g_out, g_last)
         q, k, v, decay, memory, lengths = ctx.saved_tensors
         need_q, need_k, need_v, _, need_m = ctx.needs_input_grad[:5]
         dq, dk, dv, dm = cops.decay_attention_backward(
@@ -327,5 +345,6 @@ class DropoutFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx: Any, g):
         (seed,) = ctx.saved_tensors
+        refuse_tangents("the gradient of dropout", g)
         again = DropoutFunction.apply if torch.is_grad_enabled() else cops.dropout
         return again(g, seed, *ctx.cfg), None, None, None

@@ -16,7 +16,7 @@ import torch
 
 from myelin_b200 import _native as nat
 from myelin_b200 import compile_ops as cops
-from myelin_b200.autograd import DropoutFunction
+from myelin_b200.autograd import DropoutFunction, refuse_tangents, wants_grad
 
 DRAW_RANGE = 65536  # 16 random bits per element
 
@@ -59,6 +59,7 @@ def spike_dropout(
     if seed.device != inputs.device:
         raise ValueError("seed must be on the same device as inputs")
     seed = seed.contiguous()
-    if inputs.requires_grad and torch.is_grad_enabled():
+    refuse_tangents("dropout", inputs)
+    if wants_grad(inputs):
         return DropoutFunction.apply(inputs, seed, threshold, bool(time_shared))
     return cops.dropout(inputs, seed, threshold, time_shared)

@@ -18,6 +18,7 @@ import torch
 
 from myelin_b200 import _native as nat
 from myelin_b200 import compile_ops as cops
+from myelin_b200.autograd import refuse_tangents, wants_grad
 
 MAX_FEATURES = 2**17 - 1  # sums of products of bytes stay exact in int32
 
@@ -67,6 +68,7 @@ def quantize_rows(inputs: torch.Tensor) -> QuantizedRows:
         raise ValueError(f"inputs must be shaped [..., K] with K >= 1; got {tuple(inputs.shape)}")
     nat.require_cuda(inputs)
     _check_float(inputs, "inputs")
+    refuse_tangents("quantize_rows", inputs)
     K = inputs.shape[-1]
     data, scale = cops.quantize_rows(inputs.detach().reshape(-1, K))
     return QuantizedRows(data.reshape(inputs.shape), scale.reshape(inputs.shape[:-1]))
@@ -80,6 +82,7 @@ def quantize_weight(weight: torch.Tensor) -> QuantizedWeight:
         raise ValueError(f"weight must be shaped [K, N] with K >= 1; got {tuple(weight.shape)}")
     nat.require_cuda(weight, "weight")
     _check_float(weight, "weight")
+    refuse_tangents("quantize_weight", weight)
     if weight.shape[0] > MAX_FEATURES:
         raise ValueError(f"at most {MAX_FEATURES} input features; got {weight.shape[0]}")
     data, scale = cops.quantize_rows(weight.detach().t().contiguous())
@@ -139,8 +142,8 @@ def quantized_linear(
         out_dtype = x.dtype if x.dtype.is_floating_point else torch.float32
     if out_dtype not in nat.SCAN_DTYPES:
         raise ValueError(f"out_dtype must be float32, bfloat16 or float16; got {out_dtype}")
-    if (x.requires_grad or weight.scale.requires_grad
-            or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
+    refuse_tangents("quantized_linear", x, scale, weight.scale, bias)
+    if wants_grad(x, weight.scale, bias):
         raise NotImplementedError("quantized_linear is forward only; detach its inputs or call "
                                   "it under torch.no_grad()")
     out = cops.quantized_project(
