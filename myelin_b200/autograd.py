@@ -344,7 +344,7 @@ class DropoutFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx: Any, g):
-        (seed,) = ctx.saved_tensors
         refuse_tangents("the gradient of dropout", g)
+        (seed,) = ctx.saved_tensors
         again = DropoutFunction.apply if torch.is_grad_enabled() else cops.dropout
         return again(g, seed, *ctx.cfg), None, None, None
