@@ -21,14 +21,14 @@ __host__ __device__ constexpr int rec_steps(int rows, int cols) {
 // (the next ones on their way meanwhile), walks them without a barrier and then adds
 // the eight warps' partial outputs.
 //
-// The leak is taken out of the inner loop: over a burst of steps p = 0, 1, ... the
-// block keeps g^-p S_p, so that a step is two FMAs per memory element (in pairs,
+// The leak is taken out of the inner loop: over a burst of steps p = 0 .. P-1 the
+// block keeps g^(P-1-p) S_p, so that a step is two FMAs per memory element (in pairs,
 // f32x2) instead of a product and two FMAs:
-//   S~ += (g^-p k_p) v_p^T,   o_p = g^p q_p^T S~,
-// with the leak of the first step applied before a forward burst, that of the last
-// one after a reverse burst. The powers are formed in double, so that g^-p g^p is 1
-// to two roundings. Decays below 0.02 (whose powers would leave fp32's range) take
-// bursts of one step. About 2 Dk Dv FMAs per step and head bound it, once a lane has
+//   S~ += (g^(P-1-p) k_p) v_p^T,   o_p = g^-(P-1-p) q_p^T S~,
+// from S~ = g^P S_-1; in reverse from g^(P-1) H, and H = g S~ after it. The
+// powers are formed in double, so that g^-i g^i is 1 to two roundings. What is kept is
+// never above the memory itself, and bursts are as long as keep g^(P-1) at 2^-15 or
+// more (burst_steps): it may round where fp32 ends, which costs the memory 2^-135. About 2 Dk Dv FMAs per step and head bound it, once a lane has
 // several columns: a broadcast 16-byte read of k or q fills a warp's registers in four
 // cycles whatever it is used for, so that with one column per lane those reads took
 // 0.906 ms at T=1024, 256 rows of 128 x 128 heads (19 TFLOP/s).
@@ -40,6 +40,15 @@ __device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
       : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
         "l"(*reinterpret_cast<uint64_t*>(&c)));
   return *reinterpret_cast<float2*>(&r);
+}
+
+// Steps of a burst: 16 down to g = 2^-1, 8 to 2^(-15/7), 4 to 2^-5, 2 to 2^-15, then 1,
+// as also for memories that grow (whose powers would overflow).
+template <int TC>
+__device__ __forceinline__ int burst_steps(float g) {
+  if (!(g <= 1.0f)) return 1;
+  const int most = g >= 0.5f ? 16 : g >= 0.2265f ? 8 : g >= 0.03125f ? 4 : g >= 0x1p-15f ? 2 : 1;
+  return most < TC ? most : TC;
 }
 
 template <typename T, int R, int C, bool STATES_ONLY>
@@ -55,7 +64,8 @@ __global__ void __launch_bounds__(kRecThreads)
   __shared__ __align__(16) float sq[STATES_ONLY ? 1 : TC][ROWS];
   __shared__ float sv[TC][kCols];
   __shared__ float part[STATES_ONLY ? 1 : TC][kRecWarps][kCols];
-  __shared__ float s_pow[TC + 1], s_inv[TC];  // g^p, g^-p
+  __shared__ float s_pow[TC + 1], s_inv[TC];  // g^i, g^-i (i < burst)
+  __shared__ float s_in[TC], s_out[TC];       // weights of a staged step's key and output
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t tiles = (a.Dv + kCols - 1) / kCols;
@@ -81,12 +91,22 @@ __global__ void __launch_bounds__(kRecThreads)
   T* o = static_cast<T*>(a.o.data) + b * a.o.stride_b + h * a.o.stride_h;
   const float g = a.decay[h];
   const bool reverse = a.reverse != 0;
-  const int burst = g >= 0.02f ? TC : 1;
+  const int burst = burst_steps<TC>(g);
+  // the weights of a group of `steps` staged steps, by their place from their burst's end
+  // (keys past the last step are zeros)
+  auto weights = [&](int steps) {
+    const int s = threadIdx.x;
+    if (s >= steps) return;
+    const int p = s & (burst - 1);
+    const int left = min(burst, steps - s + p) - 1 - p;
+    s_in[s] = s_pow[left];
+    s_out[s] = a.out_scale * s_inv[left];
+  };
   if (threadIdx.x <= TC) {
     double p = 1.0;
     for (int i = 0; i < int(threadIdx.x); ++i) p *= static_cast<double>(g);
     s_pow[threadIdx.x] = static_cast<float>(p);
-    if (threadIdx.x < TC) s_inv[threadIdx.x] = burst == 1 ? 1.0f : static_cast<float>(1.0 / p);
+    if (threadIdx.x < burst) s_inv[threadIdx.x] = threadIdx.x == 0 ? 1.0f : static_cast<float>(1.0 / p);
   }
 
   float2 S[C][R / 2];  // columns col0 + lane + 32 c
@@ -140,13 +160,22 @@ __global__ void __launch_bounds__(kRecThreads)
     }
   };
   if (n > 0) fetch(0);
+  __syncthreads();  // the powers are written
+  weights(TC);
+  const float full = s_pow[burst];
+  int untouched = reverse ? 1 : 0;
   for (int64_t p0 = 0; p0 < n; p0 += TC) {
     const int steps = static_cast<int>(imin64(TC, n - p0));
-    __syncthreads();  // the previous steps' staging has been read; the powers are written
+    __syncthreads();  // the previous steps' staging and weights have been read
+    if (steps < TC) {
+      weights(steps);
+      __syncthreads();
+    }
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
       const int e = threadIdx.x + i * kRecThreads, s = e / ROWS;
-      sk[s][e % ROWS] = rk[i] * (a.kv_scale * s_inv[s]);
+      // (rows past the last step are zeros: any weight)
+      sk[s][e % ROWS] = rk[i] * a.kv_scale * s_in[s];
       if constexpr (!STATES_ONLY) sq[s][e % ROWS] = rq[i];
     }
 #pragma unroll
@@ -158,7 +187,9 @@ __global__ void __launch_bounds__(kRecThreads)
     if (p0 + TC < n) fetch(p0 + TC);
     for (int s0 = 0; s0 < steps; s0 += burst) {
       const int s1 = min(steps, s0 + burst);
-      if (!reverse) scale_memory(g);
+      // (in reverse the leak of the last burst's last step is still to come, except the first time)
+      scale_memory(s1 - s0 == burst && !untouched ? full : s_pow[s1 - s0 - untouched]);
+      untouched = 0;
       auto step = [&](int s) {
         float2 vc[C], acc[C];
 #pragma unroll
@@ -195,7 +226,6 @@ __global__ void __launch_bounds__(kRecThreads)
       } else {
         for (int s = s0; s < s1; ++s) step(s);
       }
-      scale_memory(s_pow[reverse ? s1 - s0 : s1 - s0 - 1]);
     }
     if constexpr (!STATES_ONLY) {
       __syncthreads();
@@ -205,11 +235,12 @@ __global__ void __launch_bounds__(kRecThreads)
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kRecWarps; ++w) sum += part[s][w][c];
-        const float out = burst == 1 ? a.out_scale : a.out_scale * s_pow[s];
-        o[step_at(p0 + s) * a.o.stride_t + col0 + c] = Elem<T>::from_f(sum * out);
+        o[step_at(p0 + s) * a.o.stride_t + col0 + c] = Elem<T>::from_f(sum * s_out[s]);
       }
     }
   }
+
+  if (reverse && n > 0) scale_memory(g);
 
   if constexpr (!STATES_ONLY) {  // steps past the row's length: zeros
     const int64_t z0 = end > lo ? end : lo;

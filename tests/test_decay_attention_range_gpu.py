@@ -113,3 +113,49 @@ def test_a_memory_that_grows(dtype):
     state, out = mb.decay_attention_forward(q, k, v, decay, scale=1e-13)
     check(out, o, out_bound(A_o, dtype, T, D), "outputs")
     check(state.memory, S, memory_bound(A_S, dtype, T, D), "memory")
+
+
+@pytest.mark.parametrize("dtype, T", [(torch.float32, 45), (torch.float32, 1030),
+                                      (torch.bfloat16, 13)])
+@pytest.mark.parametrize("size", [1e16, 1.0, 1e-15])
+@pytest.mark.parametrize("D", [32, 80, 200])
+def test_fast_leaks_keep_the_range_of_fp32(D, size, dtype, T):
+    """The recurrent kernel, whose bursts of steps must not leave the range that the
+    memory itself stays in: products of 1e32 and of 1e-30 with decays down to 0.
+
+    Below fp32's normal range a kept value is rounded to a multiple of 2^-149, and it is
+    at least 2^-15 of the memory: 2^-135 of memory per step, at most T of them, for each
+    element of the operand that reads it. (1e16 puts the memory of dk at 1e-34.)"""
+
+    decay = torch.tensor([0.0, 1e-5, 0.02, 0.1, 0.24, 0.4, 0.55, 1.0], device=DEV)
+    H, scale = decay.numel(), 1.0 / (size * size * D)
+    q, k, v = ((_randn((T, 1, H, D), s) * m).to(dtype) for s, m in ((1, 1.0), (2, size), (3, size)))
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    state, out = mb.decay_attention_forward(*leaves, decay, scale=scale)
+    S, o = reference(q, k, v, decay, None, scale)
+    A_S, A_o = magnitude(q, k, v, decay, None, scale)
+    u = 2.0**-8 if dtype == torch.bfloat16 else 0.0  # the outputs' own rounding
+    fp32 = (2 * T + D + 8) * 2.0**-24
+    floor = lambda x, c: T * 2.0**-135 * c * x.detach().double().abs().sum(-1, keepdim=True)  # noqa: E731
+    check(out.detach(), o.detach(), (fp32 + u) * A_o.detach() + floor(q, scale), "outputs")
+    check(state.memory.detach(), S.detach(), fp32 * A_S.detach() + T * 2.0**-135, "memory")
+    go = _randn(out.shape, 5, dtype)
+    got = torch.autograd.grad(out, leaves, go)
+    doubles = [x.detach().double().requires_grad_(True) for x in leaves]
+    want = torch.autograd.grad(reference(*doubles, decay, None, scale)[1], doubles, go.double())
+    parts = [x.detach().double().abs().requires_grad_(True) for x in leaves]
+    sizes = torch.autograd.grad(reference(*parts, decay, None, scale)[1], parts, go.double().abs())
+    reads = (floor(go, scale), floor(v, 1.0), floor(k, 1.0))
+    for name, a, w, A, low in zip(("dq", "dk", "dv"), got, want, sizes, reads):
+        check(a, w, (fp32 + u) * A + low, name)
+
+
+def test_a_memory_that_grows_fast():
+    T, D = 20, 48
+    decay = torch.tensor([1.5, 4.0, 30.0], device=DEV)
+    q, k, v = (_randn((T, 1, 3, D), s) for s in (1, 2, 3))
+    S, o = reference(q, k, v, decay, None, 1e-3)
+    A_S, A_o = magnitude(q, k, v, decay, None, 1e-3)
+    state, out = mb.decay_attention_forward(q, k, v, decay, scale=1e-3)
+    check(out, o, out_bound(A_o, q.dtype, T, D), "outputs")
+    check(state.memory, S, memory_bound(A_S, q.dtype, T, D), "memory")
