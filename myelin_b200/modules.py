@@ -81,6 +81,13 @@ class LinearSynapse(nn.Module):
         return output
 
 
+def _keep_fp32(before: torch.Tensor, after: torch.Tensor) -> torch.Tensor:
+    """A buffer after its module was moved or cast: ``after``, or where that was cast,
+    ``before`` on its device."""
+
+    return after if after.dtype == torch.float32 else before.to(after.device)
+
+
 class QuantizedLinearSynapse(nn.Module):
     """A ``LinearSynapse`` for inference in 8-bit integers (``quantized_linear``).
 
@@ -103,7 +110,7 @@ class QuantizedLinearSynapse(nn.Module):
         # a change of dtype is for the bias; the scales stay fp32
         scale = self.scale
         super()._apply(fn, recurse)
-        self.scale = scale.to(self.scale.device)
+        self.scale = _keep_fp32(scale, self.scale)
         self.data = i8_operand(self.data)  # a move to another device drops the row pitch
         return self
 
@@ -392,7 +399,7 @@ class SpikeDropout(nn.Module):
             raise ValueError(f"dropout probability must be in [0, 1]; got {p}")
         self.p = p
         self.time_shared = time_shared
-        first = int(torch.randint(2**62, ())) if seed is None else seed
+        first = int(torch.randint(2**62, (), device="cpu")) if seed is None else seed
         self.register_buffer("rng", torch.tensor([first, 0], dtype=torch.int64))
 
     def next_seed(self) -> torch.Tensor:
@@ -469,7 +476,7 @@ class DecayAttention(nn.Module):
         # a change of dtype is for the projections; decays stay fp32
         decay = self.decay
         super()._apply(fn, recurse)
-        self.decay = decay.to(self.decay.device)
+        self.decay = _keep_fp32(decay, self.decay)
         return self
 
     def _heads(self, inputs: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
