@@ -318,7 +318,8 @@ class LinearSurrogateLIF(nn.Module):
 
     def forward(self, inputs: torch.Tensor) -> torch.Tensor:
         cell = self.unroll.cell
-        if self.stream_synapse and isinstance(self.synapse, LinearSynapse):
+        # (a quantised synapse has no float weight for the fused function)
+        if self.stream_synapse and not isinstance(self.synapse, QuantizedLinearSynapse):
             _state, spikes = linear_surrogate_lif_forward(
                 inputs,
                 self.synapse.weight,
