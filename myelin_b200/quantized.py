@@ -143,7 +143,7 @@ def quantized_linear(
     if out_dtype not in nat.SCAN_DTYPES:
         raise ValueError(f"out_dtype must be float32, bfloat16 or float16; got {out_dtype}")
     refuse_tangents("quantized_linear", x, scale, weight.scale, bias)
-    if wants_grad(x, weight.scale, bias):
+    if wants_grad(x, scale, weight.scale, bias):
         raise NotImplementedError("quantized_linear is forward only; detach its inputs or call "
                                   "it under torch.no_grad()")
     out = cops.quantized_project(
