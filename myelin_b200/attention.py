@@ -108,7 +108,8 @@ def decay_attention_forward(
     """Whole sequences: queries, keys ``[T, B, H, Dk]``, values ``[T, B, H, Dv]``.
 
     ``decay`` is fp32 ``[H]`` on the device, each value in [0, 1] (not checked:
-    that would read it back; a larger one grows, a negative one gives NaN).
+    that would read it back; a memory with a larger one grows, and what a
+    negative one gives is not defined).
     ``initial_state`` is zero without one. ``lengths`` (int32 ``[B]`` on the
     device, clamped to [0, T]) ends each batch row early: steps past it leave
     the memory alone, give zero outputs and zero gradients, and what the inputs

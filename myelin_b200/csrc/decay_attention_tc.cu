@@ -328,12 +328,13 @@ __device__ __forceinline__ int piece_at(int r, int q, int rows) {
 }
 
 // The power of two that brings `top` to [2^13, 2^14): fp16 operands keep their
-// full precision and range whatever their magnitude. 1 for zero and non-finite.
+// full precision and range whatever their magnitude (fp32's own range: the scale and its
+// inverse are normal numbers). 1 for zero and non-finite.
 __device__ __forceinline__ float fp16_scale(float top) {
   const int e = static_cast<int>((__float_as_uint(top) >> 23) & 0xff);
   if (e == 0 || e == 0xff) return 1.0f;
   int s = 127 + 13 - (e - 127);  // biased exponent of the scale
-  s = s < 67 ? 67 : (s > 187 ? 187 : s);  // 2^-60 .. 2^60
+  s = s < 14 ? 14 : (s > 240 ? 240 : s);  // 2^-113 .. 2^113
   return __uint_as_float(static_cast<uint32_t>(s) << 23);
 }
 

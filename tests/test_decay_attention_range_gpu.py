@@ -159,3 +159,22 @@ def test_a_memory_that_grows_fast():
     state, out = mb.decay_attention_forward(q, k, v, decay, scale=1e-3)
     check(out, o, out_bound(A_o, q.dtype, T, D), "outputs")
     check(state.memory, S, memory_bound(A_S, q.dtype, T, D), "memory")
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("size", [1e-30, 1e25])
+def test_memories_of_any_size(size, dtype):
+    """A first memory far from 1, brought back by the outputs' scale (no keys, so that
+    it is all there is to read)."""
+
+    T, B, H, D = 300, 2, 2, 64
+    decay = torch.tensor([0.98, 0.999], device=DEV)
+    q, v = _randn((T, B, H, D), 1, dtype), _randn((T, B, H, D), 3, dtype)
+    k, memory = torch.zeros_like(q), _randn((B, H, D, D), 4) * size
+    scale = 1.0 / (size * D)
+    state, out = mb.decay_attention_forward(q, k, v, decay, mb.DecayAttentionState(memory),
+                                            scale=scale)
+    S, o = reference(q, k, v, decay, memory, scale)
+    A_S, A_o = magnitude(q, k, v, decay, memory, scale)
+    check(out, o, out_bound(A_o, dtype, T, D), "outputs")
+    check(state.memory, S, memory_bound(A_S, dtype, T, D), "memory")
