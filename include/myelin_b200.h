@@ -550,7 +550,8 @@ int mb_quantize_rows(int dtype, const void* x, int64_t rows, int64_t cols, int64
  * on 16 bytes; bytes between K and the pitch are not used), K < 2^17 so that every
  * sum is exact in int32; a_scale fp32 [M] or NULL (1: integers, 0/1 spikes), b_scale
  * fp32 [N], bias [N] of `bias_dtype` or NULL; C of `out_dtype` (f32, bf16, f16), rows
- * ldc elements apart. One fp32 scaling, one rounding. tcgen05.mma kind::i8.
+ * ldc elements apart. The sum times b_scale, then one FMA with a_scale and bias in fp32,
+ * one rounding. tcgen05.mma kind::i8.
  * Replaces: LinearSynapse's projection (src/myelin/modules.py:112-133) for inference.
  */
 int mb_gemm_i8(const int8_t* a, int64_t lda, const float* a_scale, const int8_t* b, int64_t ldb,

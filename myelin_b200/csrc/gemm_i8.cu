@@ -213,9 +213,11 @@ __device__ __forceinline__ float load_bias(const I8Args& a, int64_t n) {
   return __half2float(static_cast<const __half*>(a.bias)[n]);
 }
 
-// One finished sum: the two scales multiplied first, then one FMA.
+// One finished sum. The channel's scale first: the scales' own product may leave fp32's
+// range where the result does not (rows of 1e-23 by weights of 1e-13), and a sum of 0 by
+// an infinite product would be NaN.
 __device__ __forceinline__ float scaled(int32_t acc, float sa, float sb, float bias) {
-  return fmaf(static_cast<float>(acc), sa * sb, bias);
+  return fmaf(static_cast<float>(acc) * sb, sa, bias);
 }
 
 // ---------------------------------------------------------------------------
