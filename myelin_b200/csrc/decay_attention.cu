@@ -161,13 +161,13 @@ __global__ void __launch_bounds__(kRecThreads)
   };
   if (n > 0) fetch(0);
   __syncthreads();  // the powers are written
-  weights(TC);
+  weights(static_cast<int>(imin64(TC, n)));
   const float full = s_pow[burst];
   int untouched = reverse ? 1 : 0;
   for (int64_t p0 = 0; p0 < n; p0 += TC) {
     const int steps = static_cast<int>(imin64(TC, n - p0));
     __syncthreads();  // the previous steps' staging and weights have been read
-    if (steps < TC) {
+    if (steps < TC && p0 > 0) {
       weights(steps);
       __syncthreads();
     }
