@@ -463,7 +463,12 @@ int mb_count_columns_noalloc(const int32_t* words, int64_t rows, int64_t n, int6
  * four element strides. Head sizes 1..256. The three gradients are calls of the
  * same function: dq from (do, v, k) forward, dk from (v, do, q) and dv from
  * (k, q, do) in reverse.
- * Sums and memories are fp32. The result does not depend on other rows.
+ * Sums and memories are fp32. For 16-bit types, heads up to 128 and T >= 16 the
+ * products run on the tensor cores, where the weighed scores and the memory that a
+ * chunk of 128 steps starts from are rounded to the type (outputs within 4 half steps
+ * of their terms' magnitudes); the memories that leave are good to fp32 either way.
+ * A row's result does not depend on what other rows hold. Its rounding may depend on
+ * how many there are: B and H choose the segments of the time axis and the tile.
  * Workspace: mb_decay_attention_workspace_bytes(args) bytes (0 when the time axis
  * is not split); calls that may overlap need their own.
  * No counterpart in the reference.

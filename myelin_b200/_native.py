@@ -198,7 +198,7 @@ def _launch(name: str, device: int, *args: object) -> None:
 
 def device_status(clear: bool = True) -> int:
     """Return (and by default clear) the device status of every kernel with
-    bounded waits (scan forward/backward, both tensor-core GEMMs)."""
+    bounded waits (scan forward/backward, the tensor-core GEMMs, decayed attention)."""
 
     return int(lib().mb_device_status(1 if clear else 0))
 

@@ -115,7 +115,11 @@ def decay_attention_forward(
     the memory alone, give zero outputs and zero gradients, and what the inputs
     hold there (NaN included) is never used. Returns the state after each row's
     last step and the outputs ``[T, B, H, Dv]`` in the inputs' dtype; sums and
-    memories are fp32.
+    memories are fp32. From 16 steps on, 16-bit inputs run on the tensor cores
+    (heads up to 128), which round the weighed scores and the carried memory to
+    the inputs' dtype where they read them: the outputs' error is then 1.4 times
+    that of one rounding. A row's bits may also depend on the batch's size, which
+    chooses how the time axis is split.
 
     Gradients flow to queries, keys, values and the initial memory, from the
     outputs and the final memory. Any strides are read in place when the head
