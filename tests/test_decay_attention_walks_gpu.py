@@ -92,3 +92,35 @@ def _workspace(T, B, H, Dk, Dv, dtype):
         x.data_ptr(), *v[1:], x.data_ptr(), *v[1:], x.data_ptr(), 0, *nat._NO_MEMORY,
         *nat._NO_MEMORY, 1.0, 1.0)
     return nat.lib().mb_decay_attention_workspace_bytes(args)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T, B, H", [(200, 3, 2), (200, 80, 4), (5, 3, 2), (9000, 1, 2)])
+def test_no_row_has_a_step(T, B, H, dtype):
+    """Lengths that leave every row empty, NaN everywhere behind them."""
+
+    D = 64
+    lengths = torch.zeros(B, dtype=torch.int32, device=DEV)
+    leaves = [torch.full((T, B, H, D), float("nan"), dtype=dtype, device=DEV) for _ in range(3)]
+    leaves.append(_randn((B, H, D, D), 4))
+    leaves = [x.requires_grad_(True) for x in leaves]
+    state, out = mb.decay_attention_forward(*leaves[:3], _decays(H),
+                                            mb.DecayAttentionState(leaves[3]), lengths=lengths)
+    gm = _randn((B, H, D, D), 6)
+    got = torch.autograd.grad((out, state.memory), leaves, (torch.full_like(out, float("nan")), gm))
+    assert torch.equal(state.memory, leaves[3]) and torch.equal(got[3], gm)
+    for x in (out, *got[:3]):
+        assert torch.count_nonzero(x) == 0
+    assert nat.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_overlapping_windows_are_read_in_place(dtype):
+    """Steps that overlap in memory (a sliding window over one recording)."""
+
+    T, B, H, D = 150, 2, 2, 64
+    base = _randn((T * 16 + B * H * D,), 1, dtype)
+    view = base.as_strided((T, B, H, D), (16, H * D, D, 1))
+    want = mb.decay_attention_forward(*(view.contiguous(),) * 3, _decays(H), scale=0.01)
+    got = mb.decay_attention_forward(view, view, view, _decays(H), scale=0.01)
+    assert torch.equal(got[1], want[1]) and torch.equal(got[0].memory, want[0].memory)
