@@ -57,3 +57,33 @@ def test_compiled_layer_counts_its_calls():
         want = net(x)[1]
         assert (out - want).abs().max() <= 1e-4 * want.abs().max()
     assert not torch.equal(outs[0], outs[1])
+
+
+def test_compiled_training_step_has_the_forwards_mask():
+    torch.manual_seed(0)
+    net = mb.DecayAttention(32, 2, 16, dropout=0.5).to(DEV)
+    x = torch.randn((20, 2, 32), device=DEV, requires_grad=True)
+    fast = torch.compile(net, fullgraph=True)
+    y, got = _grads(net, x, lambda z: fast(z)[1])
+    assert net.dropout.rng[1] == 1
+    net.dropout.rng[1] = 0
+    want_y, want = _grads(net, x, lambda z: net(z)[1])
+    for a, b in zip((y, *got), (want_y, *want)):
+        assert (a - b).abs().max() <= 1e-4 * b.abs().max()
+
+
+def test_compiled_checkpoint_is_right_or_refused():
+    torch.manual_seed(0)
+    net = mb.DecayAttention(32, 2, 16, dropout=0.5).to(DEV)
+    x = torch.randn((20, 2, 32), device=DEV, requires_grad=True)
+    fast = torch.compile(lambda z: checkpoint(lambda w: net(w)[1], z, use_reentrant=False))
+    try:
+        y, got = _grads(net, x, fast)
+    except Exception as error:  # noqa: BLE001  (the compiler may wrap it)
+        assert "run again inside a backward pass" in str(error) or "HigherOrder" in str(error) \
+            or "side effect" in str(error).lower()
+        return
+    net.dropout.rng[1] = 0
+    want_y, want = _grads(net, x, lambda z: net(z)[1])
+    for a, b in zip((y, *got), (want_y, *want)):
+        assert (a - b).abs().max() <= 1e-4 * b.abs().max()
